@@ -537,6 +537,97 @@ int unetmi_comm_world(void);
 int unetmi_allreduce_f32(float* buf, size_t n, void* stream);
 int unetmi_comm_destroy(void);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Sequence operators with the channels innermost: activations [batch, length, channels], fp32 or bfloat16
+ * (UNETMI_DTYPE_*), parameters fp32.  Inputs may be slices of wider tensors: strides are in elements, the last axis is
+ * dense.  Outputs are dense.  `lengths` (device int32 [batch], values outside 0..length are held inside; NULL: all
+ * `length`) ends each sequence: outputs and gradients behind the end are zero, what the inputs hold there is not used, and
+ * a final state is the state at the end.  They stand beside the LSTM / GRU recurrences above (the sequence layers of
+ * ResUNet.py:186-197, DSUNet.py:281-312); the reference has no layer of this kind.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Short causal convolution along time, per channel:
+ *     y_t = act(bias + sum_k weight[c][k] x_{t-taps+1+k})          taps 2..4, act UNETMI_ACT_NONE or UNETMI_ACT_SILU
+ * state [batch, taps-1, channels] (activations' type): the inputs before the first (NULL: zeros).  state_out (may be NULL):
+ * the last taps-1 inputs of [state, x up to the sequence's end]; it must not be `state`. */
+typedef struct UnetmiSeqConvDesc {
+    int32_t batch, length, channels, taps, act, dtype;
+    int64_t x_stride[2];     /* between sequences, between steps */
+    int64_t dy_stride[2];    /* of the output's gradient (backward only) */
+} UnetmiSeqConvDesc;
+
+int unetmi_seq_conv_fwd(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const void* state,
+                        const int32_t* lengths, void* y, void* state_out, void* stream);
+
+/* Gradients of unetmi_seq_conv_fwd: dx, dweight, dbias and, where `dstate` is not NULL, the initial state's.  dstate_out: the final state's gradient, or NULL. */
+size_t unetmi_seq_conv_bwd_workspace_bytes(const UnetmiSeqConvDesc* d);
+int unetmi_seq_conv_bwd(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const void* state,
+                        const int32_t* lengths, const void* dy, const void* dstate_out, void* dx, float* dweight, float* dbias,
+                        void* dstate, void* ws, size_t ws_bytes, void* stream);
+
+/* One token of every row (d->batch rows, x_stride[0] between them; length is not used) on a cache of streams:
+ * state [num_slots, taps-1, channels] is read and shifted in place.  slots (device int32 [batch], NULL: row i has slot i):
+ * a negative slot is a padding row (zeros out, no state touched); a slot beyond num_slots, or one that an earlier row of the
+ * same call has, gives a row of NaN and touches no state. */
+int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const int32_t* slots,
+                         int num_slots, void* state, void* y, void* stream);
+
+/* Selective state space scan:
+ *     dt = softplus(dt_raw + dt_bias)   (softplus = 0: dt_raw + dt_bias)
+ *     h_t = exp(dt_t A) h_{t-1} + dt_t x_t B_t,     y_t = (C_t . h_t + D x_t) silu(z_t)
+ * x, dt_raw, z [batch, length, channels]; A [channels, state], state <= 64; B, C [batch, length, groups, state], channels
+ * g*channels/groups .. of group g; D, dt_bias [channels]; D, z, dt_bias may be NULL.  State [batch, channels, state] fp32
+ * (NULL: zeros); state_out may be NULL and must not be `state`.  marks (NULL for inference): the states that the backward
+ * call starts its tiles from, unetmi_ssm_scan_marks_bytes of them.  States, decays and sums are fp32 throughout. */
+typedef struct UnetmiScanDesc {
+    int32_t batch, length, channels, state, groups, dtype, softplus, reserved;
+    int64_t x_stride[2], dt_stride[2], z_stride[2], dy_stride[2];    /* between sequences, between steps */
+    int64_t b_stride[3], c_stride[3];                                /* between sequences, steps, groups */
+} UnetmiScanDesc;
+
+size_t unetmi_ssm_scan_marks_bytes(const UnetmiScanDesc* d);
+size_t unetmi_ssm_scan_fwd_workspace_bytes(const UnetmiScanDesc* d);
+int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
+                        const float* D, const void* z, const float* dt_bias, const float* state, const int32_t* lengths, void* y,
+                        float* state_out, float* marks, void* ws, size_t ws_bytes, void* stream);
+
+/* Gradients of unetmi_ssm_scan_fwd from the marks of that call.  dD and ddt_bias are written
+ * also without D and dt_bias.  dstate_out: the final state's gradient or NULL; dstate: the initial state's, or NULL.  Sums over channels
+ * and sequences are taken in a fixed order: equal calls give equal bits. */
+size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d);
+int unetmi_ssm_scan_bwd(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
+                        const float* D, const void* z, const float* dt_bias, const int32_t* lengths, const float* marks, const void* dy,
+                        const float* dstate_out, void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, float* ddt_bias,
+                        void* dz, float* dstate, void* ws, size_t ws_bytes, void* stream);
+
+/* One token of every row on a cache of streams: state [num_slots, channels, state] is advanced in place; slots as in
+ * unetmi_seq_conv_step. */
+int unetmi_ssm_scan_step(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
+                         const float* D, const void* z, const float* dt_bias, const int32_t* slots, int num_slots, float* state,
+                         void* y, void* stream);
+
+/* What stands between two blocks of a residual stream, rows [rows, channels], channels <= 8192; any part may be NULL:
+ *     u = x silu(gate);  p = post_weight u / rms(u);  r = residual + scale p;  n = pre_weight r / rms(r)
+ * rms(v) = sqrt(mean(v^2) + eps).  Without a residual the output is p, and scale and pre_weight must be NULL.  The residual
+ * stream (residual, r) may be fp32 beside bfloat16 activations (residual_dtype). */
+typedef struct UnetmiNormDesc {
+    int64_t rows;
+    int32_t channels, dtype, residual_dtype;
+    float eps;
+    int64_t x_stride, gate_stride, residual_stride;                  /* between rows */
+} UnetmiNormDesc;
+
+int unetmi_block_norm_fwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
+                          const float* scale, const float* pre_weight, void* out, void* out_norm, void* stream);
+
+/* Gradients.  stream_out: the forward call's r (needed with pre_weight; residual_stride is its row stride); d_out / d_norm:
+ * the gradients of r (or p) and n, NULL for zero.  dresidual must be given where there was a residual.  dweights: one buffer
+ * [3, channels]: post_weight, scale, pre_weight. */
+size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d);
+int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* stream_out,
+                          const float* scale, const float* pre_weight, const void* d_out, const void* d_norm, void* dx, void* dgate,
+                          void* dresidual, float* dweights, void* ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,19 @@ EXPORTED_SYMBOLS = (
     "unetmi_comm_world",
     "unetmi_allreduce_f32",
     "unetmi_comm_destroy",
+    "unetmi_seq_conv_fwd",
+    "unetmi_seq_conv_bwd_workspace_bytes",
+    "unetmi_seq_conv_bwd",
+    "unetmi_seq_conv_step",
+    "unetmi_ssm_scan_marks_bytes",
+    "unetmi_ssm_scan_fwd_workspace_bytes",
+    "unetmi_ssm_scan_fwd",
+    "unetmi_ssm_scan_bwd_workspace_bytes",
+    "unetmi_ssm_scan_bwd",
+    "unetmi_ssm_scan_step",
+    "unetmi_block_norm_fwd",
+    "unetmi_block_norm_bwd_workspace_bytes",
+    "unetmi_block_norm_bwd",
 )
 
 
@@ -87,6 +100,25 @@ class ConvDesc(ctypes.Structure):
         "N", "C0", "C1", "H", "W", "K", "OH", "OW", "kh", "kw", "sh", "sw", "ph", "pw",
         "dh", "dw", "oph", "opw", "transposed", "in_mode", "act", "act_first",
         "act_param_per_channel", "has_gate", "has_residual")] + [("reserved", ctypes.c_int32 * 3)]
+
+
+class SeqConvDesc(ctypes.Structure):
+    """struct UnetmiSeqConvDesc."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "length", "channels", "taps", "act", "dtype")] + [
+        ("x_stride", ctypes.c_int64 * 2), ("dy_stride", ctypes.c_int64 * 2)]
+
+
+class ScanDesc(ctypes.Structure):
+    """struct UnetmiScanDesc."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "length", "channels", "state", "groups", "dtype", "softplus", "reserved")] + [
+        (n, ctypes.c_int64 * 2) for n in ("x_stride", "dt_stride", "z_stride", "dy_stride")] + [
+        (n, ctypes.c_int64 * 3) for n in ("b_stride", "c_stride")]
+
+
+class NormDesc(ctypes.Structure):
+    """struct UnetmiNormDesc."""
+    _fields_ = [("rows", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("channels", "dtype", "residual_dtype")] + [
+        ("eps", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("x_stride", "gate_stride", "residual_stride")]
 
 
 E_BAD_DESC, E_BAD_ARG, E_HIP, E_UNSUPPORTED = -1, -2, -3, -4
@@ -202,6 +234,22 @@ def _load():
     lib.unetmi_comm_world.argtypes = []
     lib.unetmi_allreduce_f32.argtypes = [fp, sz, vp]
     lib.unetmi_comm_destroy.argtypes = []
+    conv, scan, norm = ctypes.POINTER(SeqConvDesc), ctypes.POINTER(ScanDesc), ctypes.POINTER(NormDesc)
+    lib.unetmi_seq_conv_fwd.argtypes = [conv] + [vp] * 8
+    lib.unetmi_seq_conv_bwd.argtypes = [conv] + [vp] * 12 + [sz, vp]
+    lib.unetmi_seq_conv_step.argtypes = [conv] + [vp] * 4 + [ci] + [vp] * 3
+    lib.unetmi_ssm_scan_fwd.argtypes = [scan] + [vp] * 14 + [sz, vp]
+    lib.unetmi_ssm_scan_bwd.argtypes = [scan] + [vp] * 22 + [sz, vp]
+    lib.unetmi_ssm_scan_step.argtypes = [scan] + [vp] * 9 + [ci] + [vp] * 3
+    lib.unetmi_block_norm_fwd.argtypes = [norm] + [vp] * 9
+    lib.unetmi_block_norm_bwd.argtypes = [norm] + [vp] * 13 + [sz, vp]
+    for f in (lib.unetmi_seq_conv_fwd, lib.unetmi_seq_conv_bwd, lib.unetmi_seq_conv_step, lib.unetmi_ssm_scan_fwd, lib.unetmi_ssm_scan_bwd,
+              lib.unetmi_ssm_scan_step, lib.unetmi_block_norm_fwd, lib.unetmi_block_norm_bwd):
+        f.restype = ctypes.c_int
+    for f, d in ((lib.unetmi_seq_conv_bwd_workspace_bytes, conv), (lib.unetmi_ssm_scan_marks_bytes, scan),
+                 (lib.unetmi_ssm_scan_fwd_workspace_bytes, scan), (lib.unetmi_ssm_scan_bwd_workspace_bytes, scan),
+                 (lib.unetmi_block_norm_bwd_workspace_bytes, norm)):
+        f.argtypes, f.restype = [d], sz
     for f in (lib.unetmi_comm_unique_id, lib.unetmi_comm_init, lib.unetmi_comm_world, lib.unetmi_allreduce_f32,
               lib.unetmi_comm_destroy):
         f.restype = ctypes.c_int

@@ -1,0 +1,343 @@
+// What stands between two blocks of a residual stream, as one pass over the rows (any part may be left out):
+//     u = x silu(gate)                 the block's gate
+//     p = w_post u / rms(u)            the norm after the block        rms(v) = sqrt(mean v^2 + eps)
+//     r = residual + scale p           the stream                      (the output p if there is no residual)
+//     n = w_pre r / rms(r)             the norm before the next block
+// Rows are read once and written once (three inputs, two outputs: ten bytes a bfloat16 element, about 16 operations), so
+// HBM bounds both directions.  A thread holds eight elements of a row in fp32; rows of up to 512 elements belong to one
+// wave, wider ones to a block of up to 16 waves.  Blocks walk over rows: the weights stay in registers, and in the
+// backward kernel so do their gradients' partial sums, added up in a fixed order by a second kernel.
+#include "seq_common.hpp"
+
+namespace unetmi {
+
+constexpr int kElems = 8;                 // row elements per thread
+
+struct NormArgs {
+    const void *x, *gate;                 // gate may be null
+    const float *post, *scale, *pre;      // null: that part is left out (scale: 1)
+    const void* residual;                 // forward: the stream; backward: its new value r
+    long long xs, gs, rs;                 // elements between rows
+    long long rows;
+    int D;
+    float eps;
+    void *out_r, *out_n;                  // r (or p without a residual), n
+    // backward
+    const void *d_r, *d_n;                // null: zero
+    void *dx, *dgate, *dres;
+    float* partial;                       // [workers, 3, D]: post, scale, pre
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x124>(v);
+    v += dpp<0x128>(v);
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// Sums over a row's threads.  One wave: no LDS.  More: the two halves of `red` are used in turn, so that one barrier per
+// call is enough.
+struct RowSum {
+    float* red;                           // [2][16][3]
+    int waves, wave, turn = 0;
+    template <int M>
+    __device__ __forceinline__ void operator()(float (&v)[M]) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
+        if (waves == 1) return;
+        float* mine = red + turn * 48;
+        turn ^= 1;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int m = 0; m < M; ++m) mine[wave * 3 + m] = v[m];
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            float s = 0.f;
+            for (int w = 0; w < waves; ++w) s += mine[w * 3 + m];
+            v[m] = s;
+        }
+    }
+};
+
+// a thread's elements of a row: NV = 8 / V vectors, `width` threads apart
+template <class T, int V>
+__device__ __forceinline__ void load_row(float (&o)[kElems], const void* p, long long row, int D, int col, int width) {
+#pragma unroll
+    for (int j = 0; j < kElems / V; ++j) {
+        const int c = (j * width + col) * V;
+        Pack<T, V> k;
+        if (c < D) k.load(static_cast<const T*>(p) + row + c);
+        else k.zero();
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[j * V + v] = k.get(v);
+    }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_row(const float (&o)[kElems], void* p, long long row, int D, int col, int width) {
+#pragma unroll
+    for (int j = 0; j < kElems / V; ++j) {
+        const int c = (j * width + col) * V;
+        Pack<T, V> k;
+#pragma unroll
+        for (int v = 0; v < V; ++v) k.set(v, o[j * V + v]);
+        if (c < D) k.store(static_cast<T*>(p) + row + c);
+    }
+}
+
+template <class T, class RT, int V>
+__global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
+    __shared__ float red[96];
+    const int width = blockDim.x, col = threadIdx.x;
+    RowSum sum{red, width >> 6, col >> 6};
+    float post[kElems], scale[kElems], pre[kElems];
+    if (a.post) load_row<float, V>(post, a.post, 0, a.D, col, width);
+    if (a.scale) load_row<float, V>(scale, a.scale, 0, a.D, col, width);
+    if (a.pre) load_row<float, V>(pre, a.pre, 0, a.D, col, width);
+    const float inv_d = 1.f / (float)a.D;
+    for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
+        float u[kElems], r[kElems];
+        load_row<T, V>(u, a.x, row * a.xs, a.D, col, width);
+        if (a.residual) load_row<RT, V>(r, a.residual, row * a.rs, a.D, col, width);
+        if (a.gate) {
+            float z[kElems];
+            load_row<T, V>(z, a.gate, row * a.gs, a.D, col, width);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
+        }
+        if (a.post) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) s[0] = fmaf(u[i], u[i], s[0]);
+            sum(s);
+            const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) u[i] *= inv * post[i];
+        }
+        if (!a.residual) {
+            store_row<T, V>(u, a.out_r, row * a.D, a.D, col, width);
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) r[i] = a.scale ? fmaf(scale[i], u[i], r[i]) : r[i] + u[i];
+        store_row<RT, V>(r, a.out_r, row * a.D, a.D, col, width);
+        if (a.pre) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) s[0] = fmaf(r[i], r[i], s[0]);
+            sum(s);
+            const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) r[i] *= inv * pre[i];
+            store_row<T, V>(r, a.out_n, row * a.D, a.D, col, width);
+        }
+    }
+}
+
+// Backward.  With f = 1 / rms(r), e = 1 / rms(u):
+//     dr = d_r + f (g - r f^2 mean(g r)),  g = d_n w_pre          dw_pre = sum_rows d_n r f
+//     dresidual = dr,  dscale = sum dr p,  dp = scale dr            (without a residual dp = d_r)
+//     du = e (q - u e^2 mean(q u)),  q = dp w_post                  dw_post = sum dp u e
+//     dx = du silu(gate),  dgate = du x silu'(gate)
+// f and e are computed again from the rows (they are read anyway); r is the stream as it was stored.
+template <class T, class RT, int V>
+__global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
+    __shared__ float red[96];
+    const int width = blockDim.x, col = threadIdx.x;
+    RowSum sum{red, width >> 6, col >> 6};
+    float post[kElems], scale[kElems], pre[kElems], d_post[kElems], d_scale[kElems], d_pre[kElems];
+#pragma unroll
+    for (int i = 0; i < kElems; ++i) { post[i] = scale[i] = 1.f; pre[i] = 0.f; d_post[i] = d_scale[i] = d_pre[i] = 0.f; }
+    if (a.post) load_row<float, V>(post, a.post, 0, a.D, col, width);
+    if (a.scale) load_row<float, V>(scale, a.scale, 0, a.D, col, width);
+    if (a.pre) load_row<float, V>(pre, a.pre, 0, a.D, col, width);
+    const float inv_d = 1.f / (float)a.D;
+    const long long worker = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    for (long long row = worker; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
+        float x[kElems], z[kElems], u[kElems], g[kElems], r[kElems], dn[kElems];
+        load_row<T, V>(x, a.x, row * a.xs, a.D, col, width);
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) { u[i] = x[i]; g[i] = 0.f; }
+        if (a.d_r) {
+            if (a.residual || a.dres) load_row<RT, V>(g, a.d_r, row * a.D, a.D, col, width);
+            else load_row<T, V>(g, a.d_r, row * a.D, a.D, col, width);
+        }
+        if (a.gate) {
+            load_row<T, V>(z, a.gate, row * a.gs, a.D, col, width);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
+        }
+        float s[3] = {0.f, 0.f, 0.f};
+        const bool with_pre = a.pre && a.d_n;
+        if (with_pre) {
+            load_row<RT, V>(r, a.residual, row * a.rs, a.D, col, width);
+            load_row<T, V>(dn, a.d_n, row * a.D, a.D, col, width);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                s[1] = fmaf(r[i], r[i], s[1]);
+                s[2] = fmaf(dn[i] * pre[i], r[i], s[2]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kElems; ++i) s[0] = fmaf(u[i], u[i], s[0]);
+        if (with_pre || a.post) sum(s);
+        const float e = a.post ? __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps)) : 1.f;
+        if (with_pre) {
+            const float f = __builtin_amdgcn_rsqf(fmaf(s[1], inv_d, a.eps)), m = f * f * s[2] * inv_d;
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
+                g[i] = fmaf(f, fmaf(-r[i], m, dn[i] * pre[i]), g[i]);
+            }
+        }
+        if (a.dres) {
+            store_row<RT, V>(g, a.dres, row * a.D, a.D, col, width);
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                d_scale[i] = fmaf(g[i], u[i] * e * post[i], d_scale[i]);
+                g[i] *= scale[i];
+            }
+        }
+        if (a.post) {
+            float q[1] = {0.f};
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                d_post[i] = fmaf(g[i], u[i] * e, d_post[i]);
+                g[i] *= post[i];
+                q[0] = fmaf(g[i], u[i], q[0]);
+            }
+            sum(q);
+            const float m = e * e * q[0] * inv_d;
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) g[i] = e * fmaf(-u[i], m, g[i]);
+        }
+        if (a.gate) {
+            float dz[kElems];
+#pragma unroll
+            for (int i = 0; i < kElems; ++i) {
+                const float sg = sigmoid_hw(z[i]);
+                dz[i] = g[i] * x[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
+                g[i] *= z[i] * sg;
+            }
+            store_row<T, V>(dz, a.dgate, row * a.D, a.D, col, width);
+        }
+        store_row<T, V>(g, a.dx, row * a.D, a.D, col, width);
+    }
+    float* out = a.partial + worker * 3 * a.D;
+    store_row<float, V>(d_post, out, 0, a.D, col, width);
+    store_row<float, V>(d_scale, out, a.D, a.D, col, width);
+    store_row<float, V>(d_pre, out, 2 * (long long)a.D, a.D, col, width);
+}
+
+namespace {
+
+struct NormPlan {
+    int width, per_block;                 // threads per row, rows per block
+    unsigned blocks;
+};
+
+NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
+    NormPlan p;
+    p.width = ((d.channels + kElems - 1) / kElems + 63) / 64 * 64;
+    p.per_block = p.width == 64 ? 4 : 1;
+    long long n = (d.rows + p.per_block - 1) / p.per_block;
+    p.blocks = (unsigned)(n < 1 ? 1 : (n > most_blocks ? most_blocks : n));
+    return p;
+}
+
+// resident work: about 32 waves per CU forward; half of that backward, whose partial sums cost 12 bytes a column and worker
+long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 32 / (p.width * p.per_block / 64); }
+long long bwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 8 / (p.width * p.per_block / 64); }
+
+bool norm_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int norm_check(const UnetmiNormDesc* d, const char* what) {
+    const std::string w = what;
+    if (!d) return api_fail(UNETMI_E_BAD_ARG, w + ": null descriptor");
+    if (d->rows < 0 || d->channels < 1) return api_fail(UNETMI_E_BAD_DESC, w + ": bad sizes");
+    if (d->channels > 8192) return api_fail(UNETMI_E_UNSUPPORTED, w + ": rows of at most 8192 elements are built");
+    if (d->dtype != UNETMI_DTYPE_F32 && d->dtype != UNETMI_DTYPE_BF16) return api_fail(UNETMI_E_UNSUPPORTED, w + ": fp32 or bfloat16 activations");
+    if (d->residual_dtype != d->dtype && d->residual_dtype != UNETMI_DTYPE_F32)
+        return api_fail(UNETMI_E_UNSUPPORTED, w + ": the residual stream is fp32 or of the activations' type");
+    if (!(d->eps >= 0.f)) return api_fail(UNETMI_E_BAD_DESC, w + ": eps must not be negative");
+    if (d->x_stride < 0 || d->gate_stride < 0 || d->residual_stride < 0) return api_fail(UNETMI_E_BAD_DESC, w + ": negative stride");
+    return UNETMI_OK;
+}
+
+template <class T, class RT, int V, bool BWD>
+int norm_launch(const NormArgs& a, const NormPlan& p, hipStream_t s) {
+    const dim3 block(p.width, p.per_block);
+    if (BWD) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, V>), dim3(p.blocks), block, 0, s, a);
+    else hipLaunchKernelGGL((block_norm_fwd_kernel<T, RT, V>), dim3(p.blocks), block, 0, s, a);
+    return launched(BWD ? "block_norm_bwd" : "block_norm_fwd");
+}
+
+template <bool BWD>
+int norm_dispatch(const UnetmiNormDesc& d, const NormArgs& a, const NormPlan& p, std::initializer_list<const void*> ptrs, hipStream_t s) {
+    const int v = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
+    bool vec = d.channels % v == 0 && a.xs % v == 0 && a.gs % v == 0 && a.rs % v == 0;
+    for (const void* q : ptrs) vec = vec && norm_aligned(q);
+    if (d.dtype == UNETMI_DTYPE_F32) return vec ? norm_launch<float, float, 4, BWD>(a, p, s) : norm_launch<float, float, 1, BWD>(a, p, s);
+    if (d.residual_dtype == UNETMI_DTYPE_F32)
+        return vec ? norm_launch<__bf16, float, 8, BWD>(a, p, s) : norm_launch<__bf16, float, 1, BWD>(a, p, s);
+    return vec ? norm_launch<__bf16, __bf16, 8, BWD>(a, p, s) : norm_launch<__bf16, __bf16, 1, BWD>(a, p, s);
+}
+
+NormArgs norm_args(const UnetmiNormDesc& d, const void* x, const void* gate, const float* post, const void* residual, const float* scale,
+                   const float* pre) {
+    NormArgs a = {};
+    a.x = x; a.gate = gate; a.post = post; a.residual = residual; a.scale = scale; a.pre = pre;
+    a.xs = d.x_stride; a.gs = gate ? d.gate_stride : 0; a.rs = residual ? d.residual_stride : 0;
+    a.rows = d.rows; a.D = d.channels; a.eps = d.eps;
+    return a;
+}
+
+}  // namespace
+}  // namespace unetmi
+
+using namespace unetmi;
+
+extern "C" {
+
+int unetmi_block_norm_fwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
+                          const float* scale, const float* pre_weight, void* out, void* out_norm, void* stream) {
+    const int rc = norm_check(d, "block_norm_fwd");
+    if (rc != UNETMI_OK) return rc;
+    if (d->rows == 0) return UNETMI_OK;
+    if (!x || !out || (pre_weight && !out_norm)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_fwd: null tensor pointer");
+    if (!residual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_fwd: scale and pre_weight belong to a residual stream");
+    NormArgs a = norm_args(*d, x, gate, post_weight, residual, scale, pre_weight);
+    a.out_r = out; a.out_n = out_norm;
+    return norm_dispatch<false>(*d, a, norm_plan(*d, fwd_blocks(*d)), {x, gate, post_weight, residual, scale, pre_weight, out, out_norm},
+                                static_cast<hipStream_t>(stream));
+}
+
+size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d) {
+    if (norm_check(d, "block_norm_bwd_workspace_bytes") != UNETMI_OK) return 0;
+    const NormPlan p = norm_plan(*d, bwd_blocks(*d));
+    return (size_t)p.blocks * p.per_block * 3 * d->channels * sizeof(float);
+}
+
+int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* stream_out,
+                          const float* scale, const float* pre_weight, const void* d_out, const void* d_norm, void* dx, void* dgate,
+                          void* dresidual, float* dweights, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = norm_check(d, "block_norm_bwd");
+    if (rc != UNETMI_OK) return rc;
+    if (d->rows == 0) return api_fail(UNETMI_E_BAD_DESC, "block_norm_bwd: no rows");
+    if (!x || !dx || !dweights || !ws || (gate && !dgate) || (pre_weight && d_norm && !stream_out))
+        return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: null tensor pointer");
+    if (!dresidual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: scale and pre_weight belong to a residual stream");
+    if (ws_bytes < unetmi_block_norm_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: workspace too small");
+    NormArgs a = norm_args(*d, x, gate, post_weight, stream_out, scale, pre_weight);
+    a.d_r = d_out; a.d_n = d_norm; a.dx = dx; a.dgate = dgate; a.dres = dresidual;
+    a.partial = static_cast<float*>(ws);
+    const NormPlan p = norm_plan(*d, bwd_blocks(*d));
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int done = norm_dispatch<true>(*d, a, p, {x, gate, post_weight, stream_out, scale, pre_weight, d_out, d_norm, dx, dgate, dresidual, ws}, s);
+    if (done != UNETMI_OK) return done;
+    return launch_sum_rows(a.partial, dweights, nullptr, 3 * d->channels, (int)(p.blocks * p.per_block), 3 * d->channels, s);
+}
+
+}  // extern "C"

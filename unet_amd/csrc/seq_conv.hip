@@ -1,0 +1,489 @@
+// Short causal convolution along time, channels innermost (x [batch, length, channels]):
+//     y_t = act(bias + sum_k w_k x_{t-K+1+k}),   K = 2..4, act = SiLU or none,
+// over the K-1 inputs before the first one (a state, or zeros), its gradients and its form for single tokens.
+// Two or three operations per tap against one read and one write of HBM: the traffic bounds all three kernels.  A thread
+// keeps one vector of channels (16 bytes where rows are aligned, else one element) and walks along time with the last
+// K-1 inputs in registers, so a row is read once per time segment plus K-1 rows that the caches still hold.
+#include "seq_common.hpp"
+
+namespace unetmi {
+
+struct ConvSeqArgs {
+    const void* x;
+    long long xb, xt;                  // elements between sequences / steps of x
+    const float *w, *bias;             // [D, K], [D] or null
+    const void* state;                 // [B, K-1, D] or null
+    const int* lengths;                // [B] or null
+    int B, L, D, act;
+    int steps;                         // time steps per thread
+    int cw_log2;                       // threads along the channel vectors = 1 << cw_log2
+};
+
+template <bool ACT>
+__device__ __forceinline__ float conv_act(float v) { return ACT ? v * sigmoid_hw(v) : v; }
+
+// input at time t (t < 0: the state's rows, or zero)
+template <class T, int V, int K>
+__device__ __forceinline__ Pack<T, V> conv_input(const ConvSeqArgs& a, int b, int t, int ch) {
+    Pack<T, V> p;
+    if (t >= 0) p.load(static_cast<const T*>(a.x) + b * a.xb + t * a.xt + ch);
+    else if (a.state) p.load(static_cast<const T*>(a.state) + ((size_t)b * (K - 1) + (t + K - 1)) * a.D + ch);
+    else p.zero();
+    return p;
+}
+
+template <class T, int V, int K, bool ACT>
+__global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restrict__ y, T* __restrict__ state_out) {
+    const int cw = 1 << a.cw_log2;
+    const int ch = (blockIdx.x * cw + (threadIdx.x & (cw - 1))) * V;
+    const int seg = blockIdx.y * (256 >> a.cw_log2) + (threadIdx.x >> a.cw_log2);
+    const int b = blockIdx.z;
+    if (ch >= a.D) return;
+    const int t0 = seg * a.steps, t1 = min(t0 + a.steps, a.L);
+    const int len = seq_len(a.lengths, b, a.L);
+    // the state after the sequence: the last K-1 of [state, x[:len]]; the first time segment writes it
+    if (state_out && seg == 0) {
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i)
+            conv_input<T, V, K>(a, b, len - (K - 1) + i, ch).store(state_out + ((size_t)b * (K - 1) + i) * a.D + ch);
+    }
+    if (t0 >= t1) return;
+    float w[K][V], bias[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = a.bias ? a.bias[ch + v] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][v] = a.w[(ch + v) * K + k];
+    }
+    T* out = y + ((size_t)b * a.L + t0) * a.D + ch;
+    const int tend = min(t1, len);
+    float win[K - 1][V];
+    if (t0 < tend) {
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) {
+            const Pack<T, V> p = conv_input<T, V, K>(a, b, t0 - (K - 1) + i, ch);
+#pragma unroll
+            for (int v = 0; v < V; ++v) win[i][v] = p.get(v);
+        }
+    }
+    const T* in = static_cast<const T*>(a.x) + b * a.xb + t0 * a.xt + ch;
+    int t = t0;
+    for (; t + 4 <= tend; t += 4) {                     // four rows in flight
+        Pack<T, V> r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { r[i].load(in); in += a.xt; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float x = r[i].get(v);
+                float s = bias[v];
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][v], win[k][v], s);
+                s = fmaf(w[K - 1][v], x, s);
+#pragma unroll
+                for (int k = 0; k + 1 < K - 1; ++k) win[k][v] = win[k + 1][v];
+                win[K - 2][v] = x;
+                o.set(v, conv_act<ACT>(s));
+            }
+            o.store(out);
+            out += a.D;
+        }
+    }
+    for (; t < tend; ++t) {
+        Pack<T, V> r, o;
+        r.load(in);
+        in += a.xt;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float x = r.get(v);
+            float s = bias[v];
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) s = fmaf(w[k][v], win[k][v], s);
+            s = fmaf(w[K - 1][v], x, s);
+#pragma unroll
+            for (int k = 0; k + 1 < K - 1; ++k) win[k][v] = win[k + 1][v];
+            win[K - 2][v] = x;
+            o.set(v, conv_act<ACT>(s));
+        }
+        o.store(out);
+        out += a.D;
+    }
+    Pack<T, V> zero;
+    zero.zero();
+    for (; t < t1; ++t, out += a.D) zero.store(out);    // behind the sequence's end
+}
+
+// Gradients.  A thread owns the steps [t0, t1): it adds their share of dw and db, and writes dx there, for which it
+// needs the pre-activation gradients of [t0, t1 + K-1): K-1 rows more at each end than the forward kernel.
+//     dpre_t = dy_t act'(pre_t),   dx_t = sum_k w_k dpre_{t+K-1-k},   dw_k = sum dpre_t x_{t-K+1+k},   db = sum dpre_t
+// The time segments of a block are added up through LDS and a block writes one row of partial sums [K+1][D]; a second
+// kernel adds the rows in a fixed order.
+template <class T, int V, int K, bool ACT>
+__global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const T* __restrict__ dy, long long dyb, long long dyt,
+                                                           const T* __restrict__ dstate_out, T* __restrict__ dx,
+                                                           float* __restrict__ partial) {
+    const int cw = 1 << a.cw_log2, nseg = 256 >> a.cw_log2;
+    const int lane_c = threadIdx.x & (cw - 1), row = threadIdx.x >> a.cw_log2;
+    const int ch0 = (blockIdx.x * cw + lane_c) * V;
+    const bool live = ch0 < a.D;
+    const int ch = live ? ch0 : 0;
+    const int b = blockIdx.z;
+    const int t0 = min((int)(blockIdx.y * nseg + row) * a.steps, a.L), t1 = min(t0 + a.steps, a.L);
+    const int len = seq_len(a.lengths, b, a.L);
+    float w[K][V], bias[V], dw[K][V], db[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = a.bias ? a.bias[ch + v] : 0.f;
+        db[v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) { w[k][v] = a.w[(ch + v) * K + k]; dw[k][v] = 0.f; }
+    }
+    const int tend = min(t1, len);
+    T* out = dx + ((size_t)b * a.L) * a.D + ch;
+    if (live && t0 < tend) {
+        float win[K - 1][V], dp[K - 1][V];
+#pragma unroll
+        for (int i = 0; i < K - 1; ++i) {
+            const Pack<T, V> p = conv_input<T, V, K>(a, b, t0 - (K - 1) + i, ch);
+#pragma unroll
+            for (int v = 0; v < V; ++v) { win[i][v] = p.get(v); dp[i][v] = 0.f; }
+        }
+        const T* in = static_cast<const T*>(a.x) + b * a.xb + t0 * a.xt + ch;
+        const T* gin = dy + b * dyb + t0 * dyt + ch;
+        // step t brings dpre_t; dx_{t-K+1} is then complete
+        for (int t = t0; t < tend + K - 1; ++t) {
+            Pack<T, V> r, g;
+            r.zero();
+            g.zero();
+            if (t < len) { r.load(in); g.load(gin); }
+            in += a.xt;
+            gin += dyt;
+            Pack<T, V> o;
+            const int to = t - (K - 1);
+            Pack<T, V> extra;
+            const int si = to - len + (K - 1);          // dx of the last K-1 inputs also comes from the state behind them
+            const bool has_extra = dstate_out && si >= 0 && to >= t0;
+            if (has_extra) extra.load(dstate_out + ((size_t)b * (K - 1) + si) * a.D + ch);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float x = r.get(v);
+                float pre = bias[v];
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k) pre = fmaf(w[k][v], win[k][v], pre);
+                pre = fmaf(w[K - 1][v], x, pre);
+                float d = g.get(v);
+                if (ACT) {
+                    const float s = sigmoid_hw(pre);
+                    d *= s * fmaf(pre, 1.f - s, 1.f);
+                }
+                if (t >= len) d = 0.f;
+                if (t < tend) {
+                    db[v] += d;
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k) dw[k][v] = fmaf(d, win[k][v], dw[k][v]);
+                    dw[K - 1][v] = fmaf(d, x, dw[K - 1][v]);
+                }
+                float sum = w[0][v] * d;                // dpre_t, dpre_{t-1}, ... meet w_0, w_1, ...
+#pragma unroll
+                for (int k = 1; k < K; ++k) sum = fmaf(w[k][v], dp[K - 1 - k][v], sum);
+                if (has_extra) sum += extra.get(v);
+                o.set(v, sum);
+#pragma unroll
+                for (int k = 0; k + 1 < K - 1; ++k) { win[k][v] = win[k + 1][v]; dp[k][v] = dp[k + 1][v]; }
+                win[K - 2][v] = x;
+                dp[K - 2][v] = d;
+            }
+            if (to >= t0) o.store(out + (size_t)to * a.D);
+        }
+    }
+    if (live) {
+        Pack<T, V> zero;
+        zero.zero();
+        for (int t = max(t0, tend); t < t1; ++t) zero.store(out + (size_t)t * a.D);
+    }
+    // add the block's time segments: [segment][tap or bias][thread along channels][V]
+    extern __shared__ float red[];
+    float* mine = red + (size_t)threadIdx.x * (K + 1) * V;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) mine[k * V + v] = dw[k][v];
+        mine[K * V + v] = db[v];
+    }
+    __syncthreads();
+    const size_t base = ((size_t)b * gridDim.y + blockIdx.y) * (size_t)a.D * (K + 1);
+    for (int e = threadIdx.x; e < cw * (K + 1) * V; e += 256) {
+        const int c = (blockIdx.x * cw + e / ((K + 1) * V)) * V + e % V;
+        if (c >= a.D) continue;
+        float s = 0.f;
+        for (int i = 0; i < nseg; ++i) s += red[(size_t)i * cw * (K + 1) * V + e];
+        const int k = (e / V) % (K + 1);
+        partial[base + (k < K ? (size_t)c * K + k : (size_t)a.D * K + c)] = s;
+    }
+}
+
+// Gradient of the initial state: row j of it is the input at time j - (K-1) < 0.
+template <class T, int K, bool ACT>
+__global__ __launch_bounds__(256) void conv_seq_dstate_kernel(ConvSeqArgs a, const T* __restrict__ dy, long long dyb, long long dyt,
+                                                              const T* __restrict__ dstate_out, T* __restrict__ dstate) {
+    const int ch = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    if (ch >= a.D) return;
+    const int len = seq_len(a.lengths, b, a.L);
+    float w[K], in[2 * K - 2], d[K - 1], g[K - 1];
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k] = a.w[ch * K + k];
+#pragma unroll
+    for (int i = 0; i < 2 * K - 2; ++i) in[i] = i - (K - 1) < len ? conv_input<T, 1, K>(a, b, i - (K - 1), ch).get(0) : 0.f;
+#pragma unroll
+    for (int t = 0; t < K - 1; ++t) {                    // the steps whose window reaches before the first input
+        float pre = a.bias ? a.bias[ch] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) pre = fmaf(w[k], in[t + k], pre);
+        float v = t < len ? widen(dy[b * dyb + t * dyt + ch]) : 0.f;
+        if (ACT) {
+            const float s = sigmoid_hw(pre);
+            v *= s * fmaf(pre, 1.f - s, 1.f);
+        }
+        d[t] = t < len ? v : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) {
+        g[j] = 0.f;
+#pragma unroll
+        for (int t = 0; t <= j; ++t) g[j] = fmaf(w[j - t], d[t], g[j]);
+        const int si = j - len;                          // a short sequence leaves rows of the old state in the new one
+        if (dstate_out && si >= 0) g[j] += widen(dstate_out[((size_t)b * (K - 1) + si) * a.D + ch]);
+        dstate[((size_t)b * (K - 1) + j) * a.D + ch] = (T)g[j];
+    }
+}
+
+// One token of every row: the window is the slot's K-1 old inputs and the new one; the slot is shifted in place.
+template <class T, int V, int K, bool ACT>
+__global__ __launch_bounds__(256) void conv_seq_step_kernel(const T* __restrict__ x, long long xb, const float* __restrict__ w,
+                                                            const float* __restrict__ bias, const int* __restrict__ slots,
+                                                            int nslots, T* __restrict__ state, T* __restrict__ y, int D) {
+    const int row = blockIdx.y;
+    bool bad;
+    const int slot = claim_slot(slots, row, nslots, &bad);
+    const int ch = (blockIdx.x * 256 + threadIdx.x) * V;
+    if (ch >= D) return;
+    Pack<T, V> o;
+    if (bad || slot < 0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) o.set(v, bad ? __builtin_nanf("") : 0.f);
+        o.store(y + (size_t)row * D + ch);
+        return;
+    }
+    T* st = state + (size_t)slot * (K - 1) * D + ch;
+    Pack<T, V> r[K];
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) r[i].load(st + (size_t)i * D);
+    r[K - 1].load(x + row * xb + ch);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float s = bias ? bias[ch + v] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) s = fmaf(w[(ch + v) * K + k], r[k].get(v), s);
+        o.set(v, conv_act<ACT>(s));
+    }
+    o.store(y + (size_t)row * D + ch);
+#pragma unroll
+    for (int i = 0; i < K - 1; ++i) r[i + 1].store(st + (size_t)i * D);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// sums of partial rows (shared by the sequence operators)
+// ---------------------------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(512) void sum_rows_kernel(const float* __restrict__ rows, float* __restrict__ out,
+                                                       float* __restrict__ rest, int split, int R, int width) {
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+    float s = 0.f;
+    if (col < width)
+        for (int r = part; r < R; r += 8) s += rows[(size_t)r * width + col];
+    __shared__ float red[8][64];
+    red[part][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (part == 0 && col < width) {
+        const int c = threadIdx.x & 63;
+        *(col < split ? out + col : rest + (col - split)) = ((red[0][c] + red[1][c]) + (red[2][c] + red[3][c])) + ((red[4][c] + red[5][c]) + (red[6][c] + red[7][c]));
+    }
+}
+
+int launch_sum_rows(const float* rows, float* out, float* rest, int split, int R, int width, hipStream_t s) {
+    hipLaunchKernelGGL(sum_rows_kernel, dim3((width + 63) / 64), dim3(512), 0, s, rows, out, rest, split, R, width);
+    return launched("sum of partial rows");
+}
+
+namespace {
+
+struct ConvSeqPlan {
+    int V, cw_log2, steps, nblk_t, nblk_c;
+};
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// threads along the channels: as many (a power of two, at most a wave) as there are channel vectors; the rest of the
+// block along time.  steps = rows per thread; the launch should give every CU a few blocks, so short or narrow inputs
+// take fewer rows per thread.
+ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d, bool vec, int most_steps) {
+    ConvSeqPlan p;
+    p.V = vec ? (d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4) : 1;
+    const int nv = (d.channels + p.V - 1) / p.V;
+    p.cw_log2 = 0;
+    while ((1 << p.cw_log2) < nv && p.cw_log2 < 6) ++p.cw_log2;
+    p.nblk_c = (nv + (1 << p.cw_log2) - 1) >> p.cw_log2;
+    const int nseg = 256 >> p.cw_log2;
+    p.steps = most_steps;
+    while (p.steps > 8 && (long long)d.batch * p.nblk_c * ((d.length + p.steps * nseg - 1) / (p.steps * nseg)) < 1024) p.steps /= 2;
+    p.nblk_t = (d.length + p.steps * nseg - 1) / (p.steps * nseg);
+    return p;
+}
+
+int conv_check(const UnetmiSeqConvDesc* d, const char* what) {
+    if (!d) return api_fail(UNETMI_E_BAD_ARG, std::string(what) + ": null descriptor");
+    if (d->batch < 0 || d->length < 0 || d->channels < 1) return api_fail(UNETMI_E_BAD_DESC, std::string(what) + ": bad sizes");
+    if (d->taps < 2 || d->taps > 4) return api_fail(UNETMI_E_UNSUPPORTED, std::string(what) + ": 2, 3 or 4 taps are built");
+    if (d->act != UNETMI_ACT_NONE && d->act != UNETMI_ACT_SILU) return api_fail(UNETMI_E_UNSUPPORTED, std::string(what) + ": activation none or SiLU");
+    if (d->dtype != UNETMI_DTYPE_F32 && d->dtype != UNETMI_DTYPE_BF16) return api_fail(UNETMI_E_UNSUPPORTED, std::string(what) + ": fp32 or bfloat16 activations");
+    if (d->batch > 65535) return api_fail(UNETMI_E_UNSUPPORTED, std::string(what) + ": more than 65535 sequences");
+    if (d->channels > (1 << 24) || d->length > (1 << 28)) return api_fail(UNETMI_E_UNSUPPORTED, std::string(what) + ": more than 2^24 channels or 2^28 steps");
+    if (d->x_stride[0] < 0 || d->x_stride[1] < 0 || d->dy_stride[0] < 0 || d->dy_stride[1] < 0) return api_fail(UNETMI_E_BAD_DESC, std::string(what) + ": negative stride");
+    return UNETMI_OK;
+}
+
+ConvSeqArgs conv_args(const UnetmiSeqConvDesc& d, const ConvSeqPlan& p, const void* x, const float* w, const float* bias,
+                      const void* state, const int* lengths) {
+    ConvSeqArgs a;
+    a.x = x; a.xb = d.x_stride[0]; a.xt = d.x_stride[1];
+    a.w = w; a.bias = bias; a.state = state; a.lengths = lengths;
+    a.B = d.batch; a.L = d.length; a.D = d.channels; a.act = d.act;
+    a.steps = p.steps; a.cw_log2 = p.cw_log2;
+    return a;
+}
+
+// rows that a vector access of 16 bytes may start on
+bool conv_vectors(const UnetmiSeqConvDesc& d, std::initializer_list<const void*> ptrs, bool with_dy) {
+    const int v = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
+    bool ok = d.channels % v == 0 && d.x_stride[0] % v == 0 && d.x_stride[1] % v == 0;
+    if (with_dy) ok = ok && d.dy_stride[0] % v == 0 && d.dy_stride[1] % v == 0;
+    for (const void* p : ptrs) ok = ok && aligned16(p);
+    return ok;
+}
+
+// F<T, V, K, ACT>() for the descriptor's type, vector width, taps and activation
+template <template <class, int, int, bool> class F, class T, int V, class... A>
+int conv_taps(const UnetmiSeqConvDesc& d, A&&... args) {
+    const bool act = d.act == UNETMI_ACT_SILU;
+    switch (d.taps) {
+        case 2: return act ? F<T, V, 2, true>::run(args...) : F<T, V, 2, false>::run(args...);
+        case 3: return act ? F<T, V, 3, true>::run(args...) : F<T, V, 3, false>::run(args...);
+        default: return act ? F<T, V, 4, true>::run(args...) : F<T, V, 4, false>::run(args...);
+    }
+}
+template <template <class, int, int, bool> class F, class... A>
+int conv_dispatch(const UnetmiSeqConvDesc& d, bool vec, A&&... args) {
+    if (d.dtype == UNETMI_DTYPE_BF16) return vec ? conv_taps<F, __bf16, 8>(d, args...) : conv_taps<F, __bf16, 1>(d, args...);
+    return vec ? conv_taps<F, float, 4>(d, args...) : conv_taps<F, float, 1>(d, args...);
+}
+
+template <class T, int V, int K, bool ACT>
+struct RunFwd {
+    static int run(const ConvSeqArgs& a, const ConvSeqPlan& p, void* y, void* state_out, hipStream_t s) {
+        hipLaunchKernelGGL((conv_seq_kernel<T, V, K, ACT>), dim3(p.nblk_c, p.nblk_t > 0 ? p.nblk_t : 1, a.B), dim3(256), 0, s, a,
+                           static_cast<T*>(y), static_cast<T*>(state_out));
+        return launched("seq_conv_fwd");
+    }
+};
+template <class T, int V, int K, bool ACT>
+struct RunBwd {
+    static int run(const ConvSeqArgs& a, const ConvSeqPlan& p, const UnetmiSeqConvDesc& d, const void* dy, const void* dstate_out,
+                   void* dx, void* dstate, float* dw, float* db, float* partial, hipStream_t s) {
+        const T* g = static_cast<const T*>(dy);
+        const T* gs = static_cast<const T*>(dstate_out);
+        const int nt = p.nblk_t > 0 ? p.nblk_t : 1;
+        hipLaunchKernelGGL((conv_seq_bwd_kernel<T, V, K, ACT>), dim3(p.nblk_c, nt, a.B), dim3(256),
+                           256 * (K + 1) * V * sizeof(float), s, a, g, d.dy_stride[0], d.dy_stride[1], gs, static_cast<T*>(dx), partial);
+        int rc = launched("seq_conv_bwd");
+        if (rc != UNETMI_OK) return rc;
+        if (dstate) {
+            hipLaunchKernelGGL((conv_seq_dstate_kernel<T, K, ACT>), dim3((a.D + 255) / 256, a.B), dim3(256), 0, s, a, g,
+                               d.dy_stride[0], d.dy_stride[1], gs, static_cast<T*>(dstate));
+            rc = launched("seq_conv_bwd state");
+            if (rc != UNETMI_OK) return rc;
+        }
+        return launch_sum_rows(partial, dw, db, a.D * K, a.B * nt, a.D * (K + 1), s);
+    }
+};
+template <class T, int V, int K, bool ACT>
+struct RunStep {
+    static int run(const UnetmiSeqConvDesc& d, const void* x, const float* w, const float* bias, const int* slots, int nslots,
+                   void* state, void* y, hipStream_t s) {
+        hipLaunchKernelGGL((conv_seq_step_kernel<T, V, K, ACT>), dim3((d.channels + 256 * V - 1) / (256 * V), d.batch), dim3(256), 0, s,
+                           static_cast<const T*>(x), (long long)d.x_stride[0], w, bias, slots, nslots, static_cast<T*>(state),
+                           static_cast<T*>(y), d.channels);
+        return launched("seq_conv_step");
+    }
+};
+
+constexpr int kFwdSteps = 16, kBwdSteps = 32;
+
+}  // namespace
+}  // namespace unetmi
+
+using namespace unetmi;
+
+extern "C" {
+
+int unetmi_seq_conv_fwd(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const void* state,
+                        const int32_t* lengths, void* y, void* state_out, void* stream) {
+    const int rc = conv_check(d, "seq_conv_fwd");
+    if (rc != UNETMI_OK) return rc;
+    if (d->batch == 0) return UNETMI_OK;
+    if (!weight || (d->length > 0 && (!x || !y))) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_fwd: null tensor pointer");
+    if (d->length == 0 && !state_out) return UNETMI_OK;
+    const bool vec = conv_vectors(*d, {x, state, y, state_out}, false);
+    const ConvSeqPlan p = conv_plan(*d, vec, kFwdSteps);
+    if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_fwd: too many steps");
+    return conv_dispatch<RunFwd>(*d, vec, conv_args(*d, p, x, weight, bias, state, lengths), p, y, state_out,
+                                 static_cast<hipStream_t>(stream));
+}
+
+size_t unetmi_seq_conv_bwd_workspace_bytes(const UnetmiSeqConvDesc* d) {
+    if (conv_check(d, "seq_conv_bwd") != UNETMI_OK) return 0;
+    // the narrower accesses take at least as many blocks along time as the wide ones: room for either
+    const ConvSeqPlan p = conv_plan(*d, false, kBwdSteps), q = conv_plan(*d, true, kBwdSteps);
+    const size_t nt = (size_t)(p.nblk_t > q.nblk_t ? p.nblk_t : q.nblk_t) + 1;
+    return (size_t)(d->batch > 0 ? d->batch : 1) * nt * d->channels * (d->taps + 1) * sizeof(float);
+}
+
+int unetmi_seq_conv_bwd(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const void* state,
+                        const int32_t* lengths, const void* dy, const void* dstate_out, void* dx, float* dweight, float* dbias,
+                        void* dstate, void* ws, size_t ws_bytes, void* stream) {
+    const int rc = conv_check(d, "seq_conv_bwd");
+    if (rc != UNETMI_OK) return rc;
+    if (d->batch == 0) return api_fail(UNETMI_E_BAD_DESC, "seq_conv_bwd: empty batch");
+    if (!weight || !dweight || !dbias || !ws || (d->length > 0 && (!x || !dy || !dx)))
+        return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: null tensor pointer");
+    if (ws_bytes < unetmi_seq_conv_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: workspace too small");
+    const bool vec = conv_vectors(*d, {x, state, dy, dstate_out, dx}, true);
+    const ConvSeqPlan p = conv_plan(*d, vec, kBwdSteps);
+    if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_bwd: too many steps");
+    return conv_dispatch<RunBwd>(*d, vec, conv_args(*d, p, x, weight, bias, state, lengths), p, *d, dy, dstate_out, dx, dstate,
+                                 dweight, dbias, static_cast<float*>(ws), static_cast<hipStream_t>(stream));
+}
+
+int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const int32_t* slots,
+                         int num_slots, void* state, void* y, void* stream) {
+    const int rc = conv_check(d, "seq_conv_step");
+    if (rc != UNETMI_OK) return rc;
+    if (d->batch == 0) return UNETMI_OK;
+    if (!x || !weight || !state || !y) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_step: null tensor pointer");
+    if (num_slots < 0 || (!slots && num_slots < d->batch)) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_step: fewer slots than rows");
+    const int v = d->dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
+    const bool vec = d->channels % v == 0 && d->x_stride[0] % v == 0 && aligned16(x) && aligned16(state) && aligned16(y);
+    return conv_dispatch<RunStep>(*d, vec, *d, x, weight, bias, slots, num_slots, state, y, static_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"
