@@ -577,8 +577,10 @@ int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float*
  *     h_t = exp(dt_t A) h_{t-1} + dt_t x_t B_t,     y_t = (C_t . h_t + D x_t) silu(z_t)
  * x, dt_raw, z [batch, length, channels]; A [channels, state], state <= 64; B, C [batch, length, groups, state], channels
  * g*channels/groups .. of group g; D, dt_bias [channels]; D, z, dt_bias may be NULL.  State [batch, channels, state] fp32
- * (NULL: zeros); state_out may be NULL and must not be `state`.  marks (NULL for inference): the states that the backward
+ * (NULL: zeros); state_out may be NULL and must not be `state`.  The inputs' steps are at most UNETMI_SEQ_MAX_STEP elements
+ * apart.  marks (NULL for inference): the states that the backward
  * call starts its tiles from, unetmi_ssm_scan_marks_bytes of them.  States, decays and sums are fp32 throughout. */
+#define UNETMI_SEQ_MAX_STEP (1 << 25)
 typedef struct UnetmiScanDesc {
     int32_t batch, length, channels, state, groups, dtype, softplus, reserved;
     int64_t x_stride[2], dt_stride[2], z_stride[2], dy_stride[2];    /* between sequences, between steps */
@@ -586,7 +588,7 @@ typedef struct UnetmiScanDesc {
 } UnetmiScanDesc;
 
 size_t unetmi_ssm_scan_marks_bytes(const UnetmiScanDesc* d);
-size_t unetmi_ssm_scan_fwd_workspace_bytes(const UnetmiScanDesc* d);
+size_t unetmi_ssm_scan_fwd_workspace_bytes(const UnetmiScanDesc* d, int ragged);     /* ragged: the call has lengths */
 int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
                         const float* D, const void* z, const float* dt_bias, const float* state, const int32_t* lengths, void* y,
                         float* state_out, float* marks, void* ws, size_t ws_bytes, void* stream);
@@ -594,7 +596,7 @@ int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
 /* Gradients of unetmi_ssm_scan_fwd from the marks of that call.  dD and ddt_bias are written
  * also without D and dt_bias.  dstate_out: the final state's gradient or NULL; dstate: the initial state's, or NULL.  Sums over channels
  * and sequences are taken in a fixed order: equal calls give equal bits. */
-size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d);
+size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d, int ragged);
 int unetmi_ssm_scan_bwd(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
                         const float* D, const void* z, const float* dt_bias, const int32_t* lengths, const float* marks, const void* dy,
                         const float* dstate_out, void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, float* ddt_bias,

@@ -27,7 +27,7 @@ def test_sequence_ops_infer_shapes():
         A, B, h = torch.empty(24, 16), torch.empty(2, 37, 3, 16, dtype=x.dtype), torch.empty(2, 24, 16)
         y, s, marks = ops.ssm_scan(x, x, A, B, B, c, x, c, h, None, True, True, True)
         assert y.shape == x.shape and y.dtype == x.dtype and s.shape == h.shape and s.dtype == torch.float32
-        assert marks.shape == (2 * 3 * 24 * 16,)
+        assert marks.shape == (2 * 5 * 24 * 16,)
         out = ops.ssm_scan_bwd(x, x, A, B, B, c, x, c, None, True, marks, x, None, True)
         assert [tuple(t.shape) for t in out] == [tuple(t.shape) for t in (x, x, A, B, B, c, x, c, h)]
         assert [t.dtype for t in out] == [t.dtype for t in (x, x, A, B, B, c, x, c, h)]
@@ -93,7 +93,7 @@ def test_c_entry_points_refuse():
     refused(fwd(scan(c_stride=(0, 0, -1))), _lib.E_BAD_DESC, "stride")
     refused(fwd(scan(length=1 << 29)), _lib.E_UNSUPPORTED, "steps")
     long = scan(length=4096)
-    assert lib.unetmi_ssm_scan_fwd_workspace_bytes(ref(long)) > 0
+    assert lib.unetmi_ssm_scan_fwd_workspace_bytes(ref(long), 0) > 0
     refused(lib.unetmi_ssm_scan_fwd(ref(long), *[p] * 13, None, 0, None), _lib.E_BAD_ARG, "workspace")
     refused(lib.unetmi_ssm_scan_bwd(ref(scan()), *[None] * 22, 0, None), _lib.E_BAD_ARG, "null")
     refused(lib.unetmi_ssm_scan_bwd(ref(scan()), *[p] * 22, 0, None), _lib.E_BAD_ARG, "workspace")

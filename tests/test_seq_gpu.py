@@ -443,7 +443,7 @@ def test_refusals_on_the_device(device):
         ssm.causal_conv(x, torch.zeros(8, 4, device=device, dtype=BF16))
     with pytest.raises(ValueError, match="state"):
         ssm.causal_conv(x, torch.zeros(8, 4, device=device), state=torch.zeros(1, 2, 8, device=device))
-    with pytest.raises(ValueError, match="dt is"):
+    with pytest.raises(ValueError, match="dt must"):
         ssm.selective_scan(x, x.to(BF16), A, bc, bc)
     with pytest.raises(ValueError, match="shape"):
         ssm.selective_scan(x, x, A, bc, bc[..., :1])

@@ -4,14 +4,12 @@
 //     r = residual + scale p           the stream                      (the output p if there is no residual)
 //     n = w_pre r / rms(r)             the norm before the next block
 // Rows are read once and written once (three inputs, two outputs: ten bytes a bfloat16 element, about 16 operations), so
-// HBM bounds both directions.  A thread holds eight elements of a row in fp32; rows of up to 512 elements belong to one
-// wave, wider ones to a block of up to 16 waves.  Blocks walk over rows: the weights stay in registers, and in the
+// HBM bounds both directions.  A thread holds E elements of a row in fp32: eight, rows of up to 512 elements one wave and
+// wider ones a block of up to eight waves; sixteen beyond 4096 elements.  Blocks walk over rows: the weights stay in registers, and in the
 // backward kernel so do their gradients' partial sums, added up in a fixed order by a second kernel.
 #include "seq_common.hpp"
 
 namespace unetmi {
-
-constexpr int kElems = 8;                 // row elements per thread
 
 struct NormArgs {
     const void *x, *gate;                 // gate may be null
@@ -40,14 +38,14 @@ __device__ __forceinline__ float wave_sum(float v) {
 // Sums over a row's threads.  One wave: no LDS.  More: the two halves of `red` are used in turn, so that one barrier per
 // call is enough.
 struct RowSum {
-    float* red;                           // [2][16][3]
+    float* red;                           // [2][8][3]
     int waves, wave, turn = 0;
     template <int M>
     __device__ __forceinline__ void operator()(float (&v)[M]) {
 #pragma unroll
         for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
         if (waves == 1) return;
-        float* mine = red + turn * 48;
+        float* mine = red + turn * 24;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
@@ -62,76 +60,77 @@ struct RowSum {
     }
 };
 
-// a thread's elements of a row: NV = 8 / V vectors, `width` threads apart
-template <class T, int V>
-__device__ __forceinline__ void load_row(float (&o)[kElems], const void* p, long long row, int D, int col, int width) {
+// a thread's elements of a row: E / V vectors, `width` threads apart
+template <class T, int V, int E>
+__device__ __forceinline__ void load_row(float (&o)[E], const void* p, long long row, int D, int col, int width) {
 #pragma unroll
-    for (int j = 0; j < kElems / V; ++j) {
+    for (int j = 0; j < E / V; ++j) {
         const int c = (j * width + col) * V;
         Pack<T, V> k;
-        if (c < D) k.load(static_cast<const T*>(p) + row + c);
-        else k.zero();
+        k.zero();
+        if (c < D) k.load_n(static_cast<const T*>(p) + row + c, D - c);
 #pragma unroll
         for (int v = 0; v < V; ++v) o[j * V + v] = k.get(v);
     }
 }
-template <class T, int V>
-__device__ __forceinline__ void store_row(const float (&o)[kElems], void* p, long long row, int D, int col, int width) {
+template <class T, int V, int E>
+__device__ __forceinline__ void store_row(const float (&o)[E], void* p, long long row, int D, int col, int width) {
 #pragma unroll
-    for (int j = 0; j < kElems / V; ++j) {
+    for (int j = 0; j < E / V; ++j) {
         const int c = (j * width + col) * V;
         Pack<T, V> k;
 #pragma unroll
         for (int v = 0; v < V; ++v) k.set(v, o[j * V + v]);
-        if (c < D) k.store(static_cast<T*>(p) + row + c);
+        if (c < D) k.store_n(static_cast<T*>(p) + row + c, D - c);
     }
 }
 
-template <class T, class RT, int V>
-__global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
-    __shared__ float red[96];
+template <class T, class RT, int E>
+__global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
+    constexpr int V = kVector<T>;
+    __shared__ float red[48];
     const int width = blockDim.x, col = threadIdx.x;
     RowSum sum{red, width >> 6, col >> 6};
-    float post[kElems], scale[kElems], pre[kElems];
-    if (a.post) load_row<float, V>(post, a.post, 0, a.D, col, width);
-    if (a.scale) load_row<float, V>(scale, a.scale, 0, a.D, col, width);
-    if (a.pre) load_row<float, V>(pre, a.pre, 0, a.D, col, width);
+    float post[E], scale[E], pre[E];
+    if (a.post) load_row<float, V, E>(post, a.post, 0, a.D, col, width);
+    if (a.scale) load_row<float, V, E>(scale, a.scale, 0, a.D, col, width);
+    if (a.pre) load_row<float, V, E>(pre, a.pre, 0, a.D, col, width);
     const float inv_d = 1.f / (float)a.D;
     for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
-        float u[kElems], r[kElems];
-        load_row<T, V>(u, a.x, row * a.xs, a.D, col, width);
-        if (a.residual) load_row<RT, V>(r, a.residual, row * a.rs, a.D, col, width);
+        float u[E], r[E];
+        load_row<T, V, E>(u, a.x, row * a.xs, a.D, col, width);
+        if (a.residual) load_row<RT, V, E>(r, a.residual, row * a.rs, a.D, col, width);
         if (a.gate) {
-            float z[kElems];
-            load_row<T, V>(z, a.gate, row * a.gs, a.D, col, width);
+            float z[E];
+            load_row<T, V, E>(z, a.gate, row * a.gs, a.D, col, width);
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
+            for (int i = 0; i < E; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
         }
         if (a.post) {
             float s[1] = {0.f};
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) s[0] = fmaf(u[i], u[i], s[0]);
+            for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
             sum(s);
             const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) u[i] *= inv * post[i];
+            for (int i = 0; i < E; ++i) u[i] *= inv * post[i];
         }
         if (!a.residual) {
-            store_row<T, V>(u, a.out_r, row * a.D, a.D, col, width);
+            store_row<T, V, E>(u, a.out_r, row * a.D, a.D, col, width);
             continue;
         }
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) r[i] = a.scale ? fmaf(scale[i], u[i], r[i]) : r[i] + u[i];
-        store_row<RT, V>(r, a.out_r, row * a.D, a.D, col, width);
+        for (int i = 0; i < E; ++i) r[i] = a.scale ? fmaf(scale[i], u[i], r[i]) : r[i] + u[i];
+        store_row<RT, V, E>(r, a.out_r, row * a.D, a.D, col, width);
         if (a.pre) {
             float s[1] = {0.f};
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) s[0] = fmaf(r[i], r[i], s[0]);
+            for (int i = 0; i < E; ++i) s[0] = fmaf(r[i], r[i], s[0]);
             sum(s);
             const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) r[i] *= inv * pre[i];
-            store_row<T, V>(r, a.out_n, row * a.D, a.D, col, width);
+            for (int i = 0; i < E; ++i) r[i] *= inv * pre[i];
+            store_row<T, V, E>(r, a.out_n, row * a.D, a.D, col, width);
         }
     }
 }
@@ -142,60 +141,61 @@ __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
 //     du = e (q - u e^2 mean(q u)),  q = dp w_post                  dw_post = sum dp u e
 //     dx = du silu(gate),  dgate = du x silu'(gate)
 // f and e are computed again from the rows (they are read anyway); r is the stream as it was stored.
-template <class T, class RT, int V>
-__global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
-    __shared__ float red[96];
+template <class T, class RT, int E>
+__global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
+    constexpr int V = kVector<T>;
+    __shared__ float red[48];
     const int width = blockDim.x, col = threadIdx.x;
     RowSum sum{red, width >> 6, col >> 6};
-    float post[kElems], scale[kElems], pre[kElems], d_post[kElems], d_scale[kElems], d_pre[kElems];
+    float post[E], scale[E], pre[E], d_post[E], d_scale[E], d_pre[E];
 #pragma unroll
-    for (int i = 0; i < kElems; ++i) { post[i] = scale[i] = 1.f; pre[i] = 0.f; d_post[i] = d_scale[i] = d_pre[i] = 0.f; }
-    if (a.post) load_row<float, V>(post, a.post, 0, a.D, col, width);
-    if (a.scale) load_row<float, V>(scale, a.scale, 0, a.D, col, width);
-    if (a.pre) load_row<float, V>(pre, a.pre, 0, a.D, col, width);
+    for (int i = 0; i < E; ++i) { post[i] = scale[i] = 1.f; pre[i] = 0.f; d_post[i] = d_scale[i] = d_pre[i] = 0.f; }
+    if (a.post) load_row<float, V, E>(post, a.post, 0, a.D, col, width);
+    if (a.scale) load_row<float, V, E>(scale, a.scale, 0, a.D, col, width);
+    if (a.pre) load_row<float, V, E>(pre, a.pre, 0, a.D, col, width);
     const float inv_d = 1.f / (float)a.D;
     const long long worker = (long long)blockIdx.x * blockDim.y + threadIdx.y;
     for (long long row = worker; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
-        float x[kElems], z[kElems], u[kElems], g[kElems], r[kElems], dn[kElems];
-        load_row<T, V>(x, a.x, row * a.xs, a.D, col, width);
+        float x[E], z[E], u[E], g[E], r[E], dn[E];
+        load_row<T, V, E>(x, a.x, row * a.xs, a.D, col, width);
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) { u[i] = x[i]; g[i] = 0.f; }
+        for (int i = 0; i < E; ++i) { u[i] = x[i]; g[i] = 0.f; }
         if (a.d_r) {
-            if (a.residual || a.dres) load_row<RT, V>(g, a.d_r, row * a.D, a.D, col, width);
-            else load_row<T, V>(g, a.d_r, row * a.D, a.D, col, width);
+            if (a.residual || a.dres) load_row<RT, V, E>(g, a.d_r, row * a.D, a.D, col, width);
+            else load_row<T, V, E>(g, a.d_r, row * a.D, a.D, col, width);
         }
         if (a.gate) {
-            load_row<T, V>(z, a.gate, row * a.gs, a.D, col, width);
+            load_row<T, V, E>(z, a.gate, row * a.gs, a.D, col, width);
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
+            for (int i = 0; i < E; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
         }
         float s[3] = {0.f, 0.f, 0.f};
         const bool with_pre = a.pre && a.d_n;
         if (with_pre) {
-            load_row<RT, V>(r, a.residual, row * a.rs, a.D, col, width);
-            load_row<T, V>(dn, a.d_n, row * a.D, a.D, col, width);
+            load_row<RT, V, E>(r, a.residual, row * a.rs, a.D, col, width);
+            load_row<T, V, E>(dn, a.d_n, row * a.D, a.D, col, width);
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) {
+            for (int i = 0; i < E; ++i) {
                 s[1] = fmaf(r[i], r[i], s[1]);
                 s[2] = fmaf(dn[i] * pre[i], r[i], s[2]);
             }
         }
 #pragma unroll
-        for (int i = 0; i < kElems; ++i) s[0] = fmaf(u[i], u[i], s[0]);
+        for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
         if (with_pre || a.post) sum(s);
         const float e = a.post ? __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps)) : 1.f;
         if (with_pre) {
             const float f = __builtin_amdgcn_rsqf(fmaf(s[1], inv_d, a.eps)), m = f * f * s[2] * inv_d;
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) {
+            for (int i = 0; i < E; ++i) {
                 d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
                 g[i] = fmaf(f, fmaf(-r[i], m, dn[i] * pre[i]), g[i]);
             }
         }
         if (a.dres) {
-            store_row<RT, V>(g, a.dres, row * a.D, a.D, col, width);
+            store_row<RT, V, E>(g, a.dres, row * a.D, a.D, col, width);
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) {
+            for (int i = 0; i < E; ++i) {
                 d_scale[i] = fmaf(g[i], u[i] * e * post[i], d_scale[i]);
                 g[i] *= scale[i];
             }
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
         if (a.post) {
             float q[1] = {0.f};
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) {
+            for (int i = 0; i < E; ++i) {
                 d_post[i] = fmaf(g[i], u[i] * e, d_post[i]);
                 g[i] *= post[i];
                 q[0] = fmaf(g[i], u[i], q[0]);
@@ -211,27 +211,29 @@ __global__ __launch_bounds__(1024) void block_norm_bwd_kernel(NormArgs a) {
             sum(q);
             const float m = e * e * q[0] * inv_d;
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) g[i] = e * fmaf(-u[i], m, g[i]);
+            for (int i = 0; i < E; ++i) g[i] = e * fmaf(-u[i], m, g[i]);
         }
         if (a.gate) {
-            float dz[kElems];
+            float dz[E];
 #pragma unroll
-            for (int i = 0; i < kElems; ++i) {
+            for (int i = 0; i < E; ++i) {
                 const float sg = sigmoid_hw(z[i]);
                 dz[i] = g[i] * x[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
                 g[i] *= z[i] * sg;
             }
-            store_row<T, V>(dz, a.dgate, row * a.D, a.D, col, width);
+            store_row<T, V, E>(dz, a.dgate, row * a.D, a.D, col, width);
         }
-        store_row<T, V>(g, a.dx, row * a.D, a.D, col, width);
+        store_row<T, V, E>(g, a.dx, row * a.D, a.D, col, width);
     }
     float* out = a.partial + worker * 3 * a.D;
-    store_row<float, V>(d_post, out, 0, a.D, col, width);
-    store_row<float, V>(d_scale, out, a.D, a.D, col, width);
-    store_row<float, V>(d_pre, out, 2 * (long long)a.D, a.D, col, width);
+    store_row<float, V, E>(d_post, out, 0, a.D, col, width);
+    store_row<float, V, E>(d_scale, out, a.D, a.D, col, width);
+    store_row<float, V, E>(d_pre, out, 2 * (long long)a.D, a.D, col, width);
 }
 
 namespace {
+
+int norm_elems(const UnetmiNormDesc& d) { return d.channels <= 4096 ? 8 : 16; }
 
 struct NormPlan {
     int width, per_block;                 // threads per row, rows per block
@@ -240,7 +242,8 @@ struct NormPlan {
 
 NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
     NormPlan p;
-    p.width = ((d.channels + kElems - 1) / kElems + 63) / 64 * 64;
+    const int e = norm_elems(d);
+    p.width = ((d.channels + e - 1) / e + 63) / 64 * 64;
     p.per_block = p.width == 64 ? 4 : 1;
     long long n = (d.rows + p.per_block - 1) / p.per_block;
     p.blocks = (unsigned)(n < 1 ? 1 : (n > most_blocks ? most_blocks : n));
@@ -250,8 +253,6 @@ NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
 // resident work: about 32 waves per CU forward; half of that backward, whose partial sums cost 12 bytes a column and worker
 long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 32 / (p.width * p.per_block / 64); }
 long long bwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 8 / (p.width * p.per_block / 64); }
-
-bool norm_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int norm_check(const UnetmiNormDesc* d, const char* what) {
     const std::string w = what;
@@ -266,23 +267,21 @@ int norm_check(const UnetmiNormDesc* d, const char* what) {
     return UNETMI_OK;
 }
 
-template <class T, class RT, int V, bool BWD>
+template <class T, class RT, int E, bool BWD>
 int norm_launch(const NormArgs& a, const NormPlan& p, hipStream_t s) {
     const dim3 block(p.width, p.per_block);
-    if (BWD) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, V>), dim3(p.blocks), block, 0, s, a);
-    else hipLaunchKernelGGL((block_norm_fwd_kernel<T, RT, V>), dim3(p.blocks), block, 0, s, a);
+    if (BWD) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, E>), dim3(p.blocks), block, 0, s, a);
+    else hipLaunchKernelGGL((block_norm_fwd_kernel<T, RT, E>), dim3(p.blocks), block, 0, s, a);
     return launched(BWD ? "block_norm_bwd" : "block_norm_fwd");
 }
 
 template <bool BWD>
-int norm_dispatch(const UnetmiNormDesc& d, const NormArgs& a, const NormPlan& p, std::initializer_list<const void*> ptrs, hipStream_t s) {
-    const int v = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
-    bool vec = d.channels % v == 0 && a.xs % v == 0 && a.gs % v == 0 && a.rs % v == 0;
-    for (const void* q : ptrs) vec = vec && norm_aligned(q);
-    if (d.dtype == UNETMI_DTYPE_F32) return vec ? norm_launch<float, float, 4, BWD>(a, p, s) : norm_launch<float, float, 1, BWD>(a, p, s);
+int norm_dispatch(const UnetmiNormDesc& d, const NormArgs& a, const NormPlan& p, hipStream_t s) {
+    const bool wide = norm_elems(d) == 16;
+    if (d.dtype == UNETMI_DTYPE_F32) return wide ? norm_launch<float, float, 16, BWD>(a, p, s) : norm_launch<float, float, 8, BWD>(a, p, s);
     if (d.residual_dtype == UNETMI_DTYPE_F32)
-        return vec ? norm_launch<__bf16, float, 8, BWD>(a, p, s) : norm_launch<__bf16, float, 1, BWD>(a, p, s);
-    return vec ? norm_launch<__bf16, __bf16, 8, BWD>(a, p, s) : norm_launch<__bf16, __bf16, 1, BWD>(a, p, s);
+        return wide ? norm_launch<__bf16, float, 16, BWD>(a, p, s) : norm_launch<__bf16, float, 8, BWD>(a, p, s);
+    return wide ? norm_launch<__bf16, __bf16, 16, BWD>(a, p, s) : norm_launch<__bf16, __bf16, 8, BWD>(a, p, s);
 }
 
 NormArgs norm_args(const UnetmiNormDesc& d, const void* x, const void* gate, const float* post, const void* residual, const float* scale,
@@ -310,8 +309,7 @@ int unetmi_block_norm_fwd(const UnetmiNormDesc* d, const void* x, const void* ga
     if (!residual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_fwd: scale and pre_weight belong to a residual stream");
     NormArgs a = norm_args(*d, x, gate, post_weight, residual, scale, pre_weight);
     a.out_r = out; a.out_n = out_norm;
-    return norm_dispatch<false>(*d, a, norm_plan(*d, fwd_blocks(*d)), {x, gate, post_weight, residual, scale, pre_weight, out, out_norm},
-                                static_cast<hipStream_t>(stream));
+    return norm_dispatch<false>(*d, a, norm_plan(*d, fwd_blocks(*d)), static_cast<hipStream_t>(stream));
 }
 
 size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d) {
@@ -335,9 +333,9 @@ int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* ga
     a.partial = static_cast<float*>(ws);
     const NormPlan p = norm_plan(*d, bwd_blocks(*d));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int done = norm_dispatch<true>(*d, a, p, {x, gate, post_weight, stream_out, scale, pre_weight, d_out, d_norm, dx, dgate, dresidual, ws}, s);
+    const int done = norm_dispatch<true>(*d, a, p, s);
     if (done != UNETMI_OK) return done;
-    return launch_sum_rows(a.partial, dweights, nullptr, 3 * d->channels, (int)(p.blocks * p.per_block), 3 * d->channels, s);
+    return launch_sum_rows(a.partial, (int)(p.blocks * p.per_block), {dweights, 3 * d->channels, 1, 1}, {nullptr, 0, 1, 0}, {nullptr, 0, 1, 0}, s);
 }
 
 }  // extern "C"

@@ -2,7 +2,7 @@
 //     y_t = act(bias + sum_k w_k x_{t-K+1+k}),   K = 2..4, act = SiLU or none,
 // over the K-1 inputs before the first one (a state, or zeros), its gradients and its form for single tokens.
 // Two or three operations per tap against one read and one write of HBM: the traffic bounds all three kernels.  A thread
-// keeps one vector of channels (16 bytes where rows are aligned, else one element) and walks along time with the last
+// keeps one vector of channels (16 bytes) and walks along time with the last
 // K-1 inputs in registers, so a row is read once per time segment plus K-1 rows that the caches still hold.
 #include "seq_common.hpp"
 
@@ -26,13 +26,24 @@ __device__ __forceinline__ float conv_act(float v) { return ACT ? v * sigmoid_hw
 template <class T, int V, int K>
 __device__ __forceinline__ Pack<T, V> conv_input(const ConvSeqArgs& a, int b, int t, int ch) {
     Pack<T, V> p;
-    if (t >= 0) p.load(static_cast<const T*>(a.x) + b * a.xb + t * a.xt + ch);
-    else if (a.state) p.load(static_cast<const T*>(a.state) + ((size_t)b * (K - 1) + (t + K - 1)) * a.D + ch);
+    if (t >= 0) p.load_n(static_cast<const T*>(a.x) + b * a.xb + t * a.xt + ch, a.D - ch);
+    else if (a.state) p.load_n(static_cast<const T*>(a.state) + ((size_t)b * (K - 1) + (t + K - 1)) * a.D + ch, a.D - ch);
     else p.zero();
     return p;
 }
+// a channel vector's taps and bias
+template <int V, int K>
+__device__ __forceinline__ void conv_weights(const float* w, const float* bias, int ch, int D, float (&wk)[K][V], float (&b)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        b[v] = bias && ch + v < D ? bias[ch + v] : 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) wk[k][v] = ch + v < D ? w[(ch + v) * K + k] : 0.f;
+    }
+}
 
-template <class T, int V, int K, bool ACT>
+// TAIL: the channels are no multiple of V, the last vector of a row holds fewer.
+template <class T, int V, int K, bool ACT, bool TAIL>
 __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restrict__ y, T* __restrict__ state_out) {
     const int cw = 1 << a.cw_log2;
     const int ch = (blockIdx.x * cw + (threadIdx.x & (cw - 1))) * V;
@@ -45,16 +56,12 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
     if (state_out && seg == 0) {
 #pragma unroll
         for (int i = 0; i < K - 1; ++i)
-            conv_input<T, V, K>(a, b, len - (K - 1) + i, ch).store(state_out + ((size_t)b * (K - 1) + i) * a.D + ch);
+            conv_input<T, V, K>(a, b, len - (K - 1) + i, ch).store_n(state_out + ((size_t)b * (K - 1) + i) * a.D + ch, a.D - ch);
     }
     if (t0 >= t1) return;
+    const int n = TAIL ? a.D - ch : V;
     float w[K][V], bias[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        bias[v] = a.bias ? a.bias[ch + v] : 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) w[k][v] = a.w[(ch + v) * K + k];
-    }
+    conv_weights<V, K>(a.w, a.bias, ch, a.D, w, bias);
     T* out = y + ((size_t)b * a.L + t0) * a.D + ch;
     const int tend = min(t1, len);
     float win[K - 1][V];
@@ -71,7 +78,7 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
     for (; t + 4 <= tend; t += 4) {                     // four rows in flight
         Pack<T, V> r[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { r[i].load(in); in += a.xt; }
+        for (int i = 0; i < 4; ++i) { r[i].load_n(in, n); in += a.xt; }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             Pack<T, V> o;
@@ -87,13 +94,13 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
                 win[K - 2][v] = x;
                 o.set(v, conv_act<ACT>(s));
             }
-            o.store(out);
+            o.store_n(out, n);
             out += a.D;
         }
     }
     for (; t < tend; ++t) {
         Pack<T, V> r, o;
-        r.load(in);
+        r.load_n(in, n);
         in += a.xt;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -107,12 +114,12 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
             win[K - 2][v] = x;
             o.set(v, conv_act<ACT>(s));
         }
-        o.store(out);
+        o.store_n(out, n);
         out += a.D;
     }
     Pack<T, V> zero;
     zero.zero();
-    for (; t < t1; ++t, out += a.D) zero.store(out);    // behind the sequence's end
+    for (; t < t1; ++t, out += a.D) zero.store_n(out, n);    // behind the sequence's end
 }
 
 // Gradients.  A thread owns the steps [t0, t1): it adds their share of dw and db, and writes dx there, for which it
@@ -120,7 +127,7 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
 //     dpre_t = dy_t act'(pre_t),   dx_t = sum_k w_k dpre_{t+K-1-k},   dw_k = sum dpre_t x_{t-K+1+k},   db = sum dpre_t
 // The time segments of a block are added up through LDS and a block writes one row of partial sums [K+1][D]; a second
 // kernel adds the rows in a fixed order.
-template <class T, int V, int K, bool ACT>
+template <class T, int V, int K, bool ACT, bool TAIL>
 __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const T* __restrict__ dy, long long dyb, long long dyt,
                                                            const T* __restrict__ dstate_out, T* __restrict__ dx,
                                                            float* __restrict__ partial) {
@@ -132,13 +139,14 @@ __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const 
     const int b = blockIdx.z;
     const int t0 = min((int)(blockIdx.y * nseg + row) * a.steps, a.L), t1 = min(t0 + a.steps, a.L);
     const int len = seq_len(a.lengths, b, a.L);
+    const int n = TAIL ? a.D - ch : V;
     float w[K][V], bias[V], dw[K][V], db[V];
+    conv_weights<V, K>(a.w, a.bias, ch, a.D, w, bias);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        bias[v] = a.bias ? a.bias[ch + v] : 0.f;
         db[v] = 0.f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) { w[k][v] = a.w[(ch + v) * K + k]; dw[k][v] = 0.f; }
+        for (int k = 0; k < K; ++k) dw[k][v] = 0.f;
     }
     const int tend = min(t1, len);
     T* out = dx + ((size_t)b * a.L) * a.D + ch;
@@ -157,7 +165,7 @@ __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const 
             Pack<T, V> r, g;
             r.zero();
             g.zero();
-            if (t < len) { r.load(in); g.load(gin); }
+            if (t < len) { r.load_n(in, n); g.load_n(gin, n); }
             in += a.xt;
             gin += dyt;
             Pack<T, V> o;
@@ -165,7 +173,7 @@ __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const 
             Pack<T, V> extra;
             const int si = to - len + (K - 1);          // dx of the last K-1 inputs also comes from the state behind them
             const bool has_extra = dstate_out && si >= 0 && to >= t0;
-            if (has_extra) extra.load(dstate_out + ((size_t)b * (K - 1) + si) * a.D + ch);
+            if (has_extra) extra.load_n(dstate_out + ((size_t)b * (K - 1) + si) * a.D + ch, n);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float x = r.get(v);
@@ -195,13 +203,13 @@ __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const 
                 win[K - 2][v] = x;
                 dp[K - 2][v] = d;
             }
-            if (to >= t0) o.store(out + (size_t)to * a.D);
+            if (to >= t0) o.store_n(out + (size_t)to * a.D, n);
         }
     }
     if (live) {
         Pack<T, V> zero;
         zero.zero();
-        for (int t = max(t0, tend); t < t1; ++t) zero.store(out + (size_t)t * a.D);
+        for (int t = max(t0, tend); t < t1; ++t) zero.store_n(out + (size_t)t * a.D, n);
     }
     // add the block's time segments: [segment][tap or bias][thread along channels][V]
     extern __shared__ float red[];
@@ -235,7 +243,11 @@ __global__ __launch_bounds__(256) void conv_seq_dstate_kernel(ConvSeqArgs a, con
 #pragma unroll
     for (int k = 0; k < K; ++k) w[k] = a.w[ch * K + k];
 #pragma unroll
-    for (int i = 0; i < 2 * K - 2; ++i) in[i] = i - (K - 1) < len ? conv_input<T, 1, K>(a, b, i - (K - 1), ch).get(0) : 0.f;
+    for (int i = 0; i < 2 * K - 2; ++i) {
+        const int t = i - (K - 1);
+        in[i] = t >= 0 ? (t < len ? widen(static_cast<const T*>(a.x)[b * a.xb + t * a.xt + ch]) : 0.f)
+                       : (a.state ? widen(static_cast<const T*>(a.state)[((size_t)b * (K - 1) + i) * a.D + ch]) : 0.f);
+    }
 #pragma unroll
     for (int t = 0; t < K - 1; ++t) {                    // the steps whose window reaches before the first input
         float pre = a.bias ? a.bias[ch] : 0.f;
@@ -273,46 +285,67 @@ __global__ __launch_bounds__(256) void conv_seq_step_kernel(const T* __restrict_
     if (bad || slot < 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) o.set(v, bad ? __builtin_nanf("") : 0.f);
-        o.store(y + (size_t)row * D + ch);
+        o.store_n(y + (size_t)row * D + ch, D - ch);
         return;
     }
     T* st = state + (size_t)slot * (K - 1) * D + ch;
+    const int n = D - ch;
     Pack<T, V> r[K];
 #pragma unroll
-    for (int i = 0; i < K - 1; ++i) r[i].load(st + (size_t)i * D);
-    r[K - 1].load(x + row * xb + ch);
+    for (int i = 0; i < K - 1; ++i) r[i].load_n(st + (size_t)i * D, n);
+    r[K - 1].load_n(x + row * xb + ch, n);
+    float wk[K][V], b[V];
+    conv_weights<V, K>(w, bias, ch, D, wk, b);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        float s = bias ? bias[ch + v] : 0.f;
+        float s = b[v];
 #pragma unroll
-        for (int k = 0; k < K; ++k) s = fmaf(w[(ch + v) * K + k], r[k].get(v), s);
+        for (int k = 0; k < K; ++k) s = fmaf(wk[k][v], r[k].get(v), s);
         o.set(v, conv_act<ACT>(s));
     }
-    o.store(y + (size_t)row * D + ch);
+    o.store_n(y + (size_t)row * D + ch, n);
 #pragma unroll
-    for (int i = 0; i < K - 1; ++i) r[i + 1].store(st + (size_t)i * D);
+    for (int i = 0; i < K - 1; ++i) r[i + 1].store_n(st + (size_t)i * D, n);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // sums of partial rows (shared by the sequence operators)
 // ---------------------------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(512) void sum_rows_kernel(const float* __restrict__ rows, float* __restrict__ out,
-                                                       float* __restrict__ rest, int split, int R, int width) {
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), part = threadIdx.x >> 6;
+// 32 columns a block, the rows over 32 groups of threads, eight loads of each in flight: one row of partial sums is a few
+// thousand columns, so columns alone would leave most of the chip idle (683 rows of 3855: 24 us with 8 groups).
+__global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict__ rows, int R, SumPiece a, SumPiece b, SumPiece c) {
+    const int width = a.columns + b.columns + c.columns;
+    const int part = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int col = blockIdx.x * 32 + lane;
     float s = 0.f;
-    if (col < width)
-        for (int r = part; r < R; r += 8) s += rows[(size_t)r * width + col];
-    __shared__ float red[8][64];
-    red[part][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (part == 0 && col < width) {
-        const int c = threadIdx.x & 63;
-        *(col < split ? out + col : rest + (col - split)) = ((red[0][c] + red[1][c]) + (red[2][c] + red[3][c])) + ((red[4][c] + red[5][c]) + (red[6][c] + red[7][c]));
+    if (col < width) {
+        int r = part;
+        for (; r + 7 * 32 < R; r += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = rows[(size_t)(r + k * 32) * width + col];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += v[k];
+        }
+        for (; r < R; r += 32) s += rows[(size_t)r * width + col];
     }
+    __shared__ float red[32][33];
+    red[part][lane] = s;
+    __syncthreads();
+    if (part != 0 || col >= width) return;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) s += red[k][lane];
+    SumPiece p = a;
+    if (col >= p.columns) { col -= p.columns; p = b; }
+    if (col >= p.columns) { col -= p.columns; p = c; }
+    const int g = col / p.padded, n = col - g * p.padded;
+    if (n < p.used) p.out[(size_t)g * p.used + n] = s;
 }
 
-int launch_sum_rows(const float* rows, float* out, float* rest, int split, int R, int width, hipStream_t s) {
-    hipLaunchKernelGGL(sum_rows_kernel, dim3((width + 63) / 64), dim3(512), 0, s, rows, out, rest, split, R, width);
+int launch_sum_rows(const float* rows, int R, SumPiece a, SumPiece b, SumPiece c, hipStream_t s) {
+    const int width = a.columns + b.columns + c.columns;
+    hipLaunchKernelGGL(sum_rows_kernel, dim3((width + 31) / 32), dim3(1024), 0, s, rows, R, a, b, c);
     return launched("sum of partial rows");
 }
 
@@ -322,14 +355,12 @@ struct ConvSeqPlan {
     int V, cw_log2, steps, nblk_t, nblk_c;
 };
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
 // threads along the channels: as many (a power of two, at most a wave) as there are channel vectors; the rest of the
 // block along time.  steps = rows per thread; the launch should give every CU a few blocks, so short or narrow inputs
 // take fewer rows per thread.
-ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d, bool vec, int most_steps) {
+ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d, int most_steps) {
     ConvSeqPlan p;
-    p.V = vec ? (d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4) : 1;
+    p.V = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
     const int nv = (d.channels + p.V - 1) / p.V;
     p.cw_log2 = 0;
     while ((1 << p.cw_log2) < nv && p.cw_log2 < 6) ++p.cw_log2;
@@ -363,15 +394,6 @@ ConvSeqArgs conv_args(const UnetmiSeqConvDesc& d, const ConvSeqPlan& p, const vo
     return a;
 }
 
-// rows that a vector access of 16 bytes may start on
-bool conv_vectors(const UnetmiSeqConvDesc& d, std::initializer_list<const void*> ptrs, bool with_dy) {
-    const int v = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
-    bool ok = d.channels % v == 0 && d.x_stride[0] % v == 0 && d.x_stride[1] % v == 0;
-    if (with_dy) ok = ok && d.dy_stride[0] % v == 0 && d.dy_stride[1] % v == 0;
-    for (const void* p : ptrs) ok = ok && aligned16(p);
-    return ok;
-}
-
 // F<T, V, K, ACT>() for the descriptor's type, vector width, taps and activation
 template <template <class, int, int, bool> class F, class T, int V, class... A>
 int conv_taps(const UnetmiSeqConvDesc& d, A&&... args) {
@@ -383,16 +405,17 @@ int conv_taps(const UnetmiSeqConvDesc& d, A&&... args) {
     }
 }
 template <template <class, int, int, bool> class F, class... A>
-int conv_dispatch(const UnetmiSeqConvDesc& d, bool vec, A&&... args) {
-    if (d.dtype == UNETMI_DTYPE_BF16) return vec ? conv_taps<F, __bf16, 8>(d, args...) : conv_taps<F, __bf16, 1>(d, args...);
-    return vec ? conv_taps<F, float, 4>(d, args...) : conv_taps<F, float, 1>(d, args...);
+int conv_dispatch(const UnetmiSeqConvDesc& d, A&&... args) {
+    return d.dtype == UNETMI_DTYPE_BF16 ? conv_taps<F, __bf16, kVector<__bf16>>(d, args...) : conv_taps<F, float, kVector<float>>(d, args...);
 }
 
 template <class T, int V, int K, bool ACT>
 struct RunFwd {
     static int run(const ConvSeqArgs& a, const ConvSeqPlan& p, void* y, void* state_out, hipStream_t s) {
-        hipLaunchKernelGGL((conv_seq_kernel<T, V, K, ACT>), dim3(p.nblk_c, p.nblk_t > 0 ? p.nblk_t : 1, a.B), dim3(256), 0, s, a,
-                           static_cast<T*>(y), static_cast<T*>(state_out));
+        const dim3 grid(p.nblk_c, p.nblk_t > 0 ? p.nblk_t : 1, a.B), block(256);
+        T *out = static_cast<T*>(y), *after = static_cast<T*>(state_out);
+        if (a.D % V) hipLaunchKernelGGL((conv_seq_kernel<T, V, K, ACT, true>), grid, block, 0, s, a, out, after);
+        else hipLaunchKernelGGL((conv_seq_kernel<T, V, K, ACT, false>), grid, block, 0, s, a, out, after);
         return launched("seq_conv_fwd");
     }
 };
@@ -403,8 +426,11 @@ struct RunBwd {
         const T* g = static_cast<const T*>(dy);
         const T* gs = static_cast<const T*>(dstate_out);
         const int nt = p.nblk_t > 0 ? p.nblk_t : 1;
-        hipLaunchKernelGGL((conv_seq_bwd_kernel<T, V, K, ACT>), dim3(p.nblk_c, nt, a.B), dim3(256),
-                           256 * (K + 1) * V * sizeof(float), s, a, g, d.dy_stride[0], d.dy_stride[1], gs, static_cast<T*>(dx), partial);
+        const dim3 grid(p.nblk_c, nt, a.B), block(256);
+        const size_t lds = 256 * (K + 1) * V * sizeof(float);
+        const long long yb = d.dy_stride[0], yt = d.dy_stride[1];
+        if (a.D % V) hipLaunchKernelGGL((conv_seq_bwd_kernel<T, V, K, ACT, true>), grid, block, lds, s, a, g, yb, yt, gs, static_cast<T*>(dx), partial);
+        else hipLaunchKernelGGL((conv_seq_bwd_kernel<T, V, K, ACT, false>), grid, block, lds, s, a, g, yb, yt, gs, static_cast<T*>(dx), partial);
         int rc = launched("seq_conv_bwd");
         if (rc != UNETMI_OK) return rc;
         if (dstate) {
@@ -413,7 +439,7 @@ struct RunBwd {
             rc = launched("seq_conv_bwd state");
             if (rc != UNETMI_OK) return rc;
         }
-        return launch_sum_rows(partial, dw, db, a.D * K, a.B * nt, a.D * (K + 1), s);
+        return launch_sum_rows(partial, a.B * nt, {dw, a.D * K, 1, 1}, {db, a.D, 1, 1}, {nullptr, 0, 1, 0}, s);
     }
 };
 template <class T, int V, int K, bool ACT>
@@ -443,19 +469,16 @@ int unetmi_seq_conv_fwd(const UnetmiSeqConvDesc* d, const void* x, const float* 
     if (d->batch == 0) return UNETMI_OK;
     if (!weight || (d->length > 0 && (!x || !y))) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_fwd: null tensor pointer");
     if (d->length == 0 && !state_out) return UNETMI_OK;
-    const bool vec = conv_vectors(*d, {x, state, y, state_out}, false);
-    const ConvSeqPlan p = conv_plan(*d, vec, kFwdSteps);
+    const ConvSeqPlan p = conv_plan(*d, kFwdSteps);
     if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_fwd: too many steps");
-    return conv_dispatch<RunFwd>(*d, vec, conv_args(*d, p, x, weight, bias, state, lengths), p, y, state_out,
+    return conv_dispatch<RunFwd>(*d, conv_args(*d, p, x, weight, bias, state, lengths), p, y, state_out,
                                  static_cast<hipStream_t>(stream));
 }
 
 size_t unetmi_seq_conv_bwd_workspace_bytes(const UnetmiSeqConvDesc* d) {
     if (conv_check(d, "seq_conv_bwd") != UNETMI_OK) return 0;
-    // the narrower accesses take at least as many blocks along time as the wide ones: room for either
-    const ConvSeqPlan p = conv_plan(*d, false, kBwdSteps), q = conv_plan(*d, true, kBwdSteps);
-    const size_t nt = (size_t)(p.nblk_t > q.nblk_t ? p.nblk_t : q.nblk_t) + 1;
-    return (size_t)(d->batch > 0 ? d->batch : 1) * nt * d->channels * (d->taps + 1) * sizeof(float);
+    const ConvSeqPlan p = conv_plan(*d, kBwdSteps);
+    return (size_t)(d->batch > 0 ? d->batch : 1) * (p.nblk_t > 0 ? p.nblk_t : 1) * d->channels * (d->taps + 1) * sizeof(float);
 }
 
 int unetmi_seq_conv_bwd(const UnetmiSeqConvDesc* d, const void* x, const float* weight, const float* bias, const void* state,
@@ -467,10 +490,9 @@ int unetmi_seq_conv_bwd(const UnetmiSeqConvDesc* d, const void* x, const float* 
     if (!weight || !dweight || !dbias || !ws || (d->length > 0 && (!x || !dy || !dx)))
         return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: null tensor pointer");
     if (ws_bytes < unetmi_seq_conv_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: workspace too small");
-    const bool vec = conv_vectors(*d, {x, state, dy, dstate_out, dx}, true);
-    const ConvSeqPlan p = conv_plan(*d, vec, kBwdSteps);
+    const ConvSeqPlan p = conv_plan(*d, kBwdSteps);
     if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_bwd: too many steps");
-    return conv_dispatch<RunBwd>(*d, vec, conv_args(*d, p, x, weight, bias, state, lengths), p, *d, dy, dstate_out, dx, dstate,
+    return conv_dispatch<RunBwd>(*d, conv_args(*d, p, x, weight, bias, state, lengths), p, *d, dy, dstate_out, dx, dstate,
                                  dweight, dbias, static_cast<float*>(ws), static_cast<hipStream_t>(stream));
 }
 
@@ -481,9 +503,7 @@ int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float*
     if (d->batch == 0) return UNETMI_OK;
     if (!x || !weight || !state || !y) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_step: null tensor pointer");
     if (num_slots < 0 || (!slots && num_slots < d->batch)) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_step: fewer slots than rows");
-    const int v = d->dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
-    const bool vec = d->channels % v == 0 && d->x_stride[0] % v == 0 && aligned16(x) && aligned16(state) && aligned16(y);
-    return conv_dispatch<RunStep>(*d, vec, *d, x, weight, bias, slots, num_slots, state, y, static_cast<hipStream_t>(stream));
+    return conv_dispatch<RunStep>(*d, *d, x, weight, bias, slots, num_slots, state, y, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

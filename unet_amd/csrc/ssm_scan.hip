@@ -19,8 +19,8 @@ constexpr int kTile = 16;                 // steps per tile of the forward kerne
 constexpr int kCh = 64;                   // channels per block
 
 // steps between two saved states, = the steps the backward kernel keeps in registers
-template <int S> constexpr int mark_steps() { return S <= 4 ? 16 : 64 / S; }
-static int mark_steps_of(int S) { return S <= 4 ? 16 : 64 / S; }
+template <int S> constexpr int mark_steps() { return S <= 2 ? 16 : S == 4 ? 8 : 4; }
+static int mark_steps_of(int S) { return S <= 2 ? 16 : S == 4 ? 8 : 4; }
 
 struct ScanArgs {
     const void *x, *dt, *z, *Bm, *Cm;     // z may be null
@@ -28,7 +28,7 @@ struct ScanArgs {
     const int* lengths;
     long long xb, xt, dtb, dtt, zb, zt, bb, bt, bg, cb, ct, cg;      // element strides
     int L, D, N, Dg, tpg;                 // channels per group, blocks per group
-    int chunk, nchunk;                    // steps per chunk (a multiple of kTile)
+    int chunk, nchunk;                    // steps per chunk (a multiple of the tile's)
     int nmark;
     bool softplus;
     void* y;
@@ -39,7 +39,7 @@ struct ScanArgs {
     long long dyb, dyt;
     const float* dhT;
     void *dx, *ddt, *dz;
-    float *dh0, *pBC, *pA, *pD;           // [B, L, G, tpg, 2, 4S]; [B nchunk, D, 4S]; [B nchunk, 2, D]
+    float *dh0, *pBC, *pA;                // partial sums: [B, L, G tpg, 2, 4S]; [B nchunk, (D, 4S), (D), (D)] of A, D, bias
 };
 
 struct Place {                            // what a thread works on
@@ -89,29 +89,115 @@ __device__ __forceinline__ void store_padded(const float (&h)[S], float* p, int 
     v.store(p + q * S);
 }
 
-// B (and C) of STEPS steps from t on into LDS as fp32 [step][4S], zero beyond tend and beyond N
-template <class T, int S, int STEPS>
-__device__ __forceinline__ void stage_rows(float* lds, const void* src, long long base, long long stride, int t, int tend, int N) {
-    constexpr int NP = 4 * S;
-#pragma unroll
-    for (int e = threadIdx.x; e < STEPS * NP; e += 256) {
-        const int i = e / NP, n = e % NP;
-        lds[e] = (t + i < tend && n < N) ? widen(static_cast<const T*>(src)[base + (t + i) * stride + n]) : 0.f;
-    }
+// Rows of a sequence are reached through buffer descriptors that start at a tile's first row: the lane's offset inside a
+// tile and the uniform one of its step are 32 bits (the host refuses steps that are further apart), and an offset beyond
+// the window reads zero and stores nothing, which is how steps behind the end and dead lanes are kept out.
+constexpr int kOutside = (int)0x80000000;
+
+template <class T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const T* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, 0x7fffffff, 0x00020000);
 }
+template <class T>
+__device__ __forceinline__ T window_load(__amdgpu_buffer_rsrc_t rs, int voff, int soff) {
+    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rs, voff, soff, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rs, voff, soff, 0));
+}
+template <class T>
+__device__ __forceinline__ void window_store(T v, __amdgpu_buffer_rsrc_t rs, int voff, int soff) {
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(short, v), rs, voff, soff, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, v), rs, voff, soff, 0);
+}
+
+// A lane's steps of a tile: 4i + q of its channel, i = 0..STEPS/4-1.
+template <class T, int STEPS>
+struct Column {
+    const T* base;                        // the chunk's first row
+    long long stride;
+    int off;                              // of the lane's first element of a tile, in bytes
+    T v[STEPS / 4];
+    __device__ __forceinline__ Column(const void* p, long long sb, long long st, const Place& pl, int t0)
+        : base(static_cast<const T*>(p) + pl.b * sb + t0 * st), stride(st), off((pl.q * (int)st + pl.ch) * (int)sizeof(T)) {}
+    // steps dt .. dt+STEPS-1 of the chunk, of which `left` are there
+    __device__ __forceinline__ void load(int dt, int left, int q) {
+        const auto rs = window(base + dt * stride);
+        const int next = 4 * (int)stride * (int)sizeof(T);
+        if (left >= STEPS) {
+#pragma unroll
+            for (int i = 0; i < STEPS / 4; ++i) v[i] = window_load<T>(rs, off, i * next);
+        } else {
+#pragma unroll
+            for (int i = 0; i < STEPS / 4; ++i) v[i] = window_load<T>(rs, 4 * i + q < left ? off : kOutside, i * next);
+        }
+    }
+};
+// the same for a dense output [.., D]
+template <class T, int STEPS>
+struct OutColumn {
+    T* base;
+    int D, off;
+    bool live;
+    __device__ __forceinline__ OutColumn(void* p, int D, size_t first_row, const Place& pl)
+        : base(static_cast<T*>(p) + first_row * D), D(D), off((pl.q * D + pl.ch) * (int)sizeof(T)), live(pl.live) {}
+    __device__ __forceinline__ void store(int dt, int left, int q, int i, float f) const {
+        window_store<T>((T)f, window(base + (size_t)dt * D), live && 4 * i + q < left ? off : kOutside, 4 * i * D * (int)sizeof(T));
+    }
+};
+
+// B or C of a tile of steps, on its way from HBM to LDS: [step][4S] as fp32, zero behind the end and beyond N
+template <class T, int S, int STEPS>
+struct Shared {
+    static constexpr int NP = 4 * S, E = (STEPS * NP + 255) / 256, ROWS = 256 / NP;
+    const T* base;
+    long long stride;
+    int off, row;                         // of the thread's first element of a tile; its step
+    T v[E];
+    __device__ __forceinline__ Shared(const void* p, long long sb, long long st, long long sg, const Place& pl, int t0, int N)
+        : base(static_cast<const T*>(p) + pl.b * sb + pl.g * sg + t0 * st), stride(st), row(threadIdx.x / NP) {
+        const int n = threadIdx.x % NP;
+        off = n < N ? (row * (int)st + n) * (int)sizeof(T) : kOutside;
+    }
+    __device__ __forceinline__ void load(int dt, int left) {
+        const auto rs = window(base + dt * stride);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int i = row + k * ROWS;
+            v[k] = window_load<T>(rs, i < left && i < STEPS ? off : kOutside, k * ROWS * (int)stride * (int)sizeof(T));
+        }
+    }
+    __device__ __forceinline__ void store(float* lds) const {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            const int e = threadIdx.x + 256 * k;
+            if (STEPS * NP % 256 == 0 || e < STEPS * NP) lds[e] = widen(v[k]);
+        }
+    }
+};
 
 template <class T>
 __device__ __forceinline__ float at(const void* p, long long i) { return widen(static_cast<const T*>(p)[i]); }
 
 // Forward.  STATE_ONLY: the first pass over a time axis that is split into chunks: the chunk's last state from zero and
 // the sum of its steps (the product of its decays is exp(A sum dt)).  Else the whole operator on a chunk, starting from
-// the states of the chunks before it.
+// the states of the chunks before it.  A tile's inputs are loaded while the tile before it is computed, B and C into the
+// other half of LDS: one barrier a tile.
 template <class T, int S, bool STATE_ONLY>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
     constexpr int NP = 4 * S, MK = mark_steps<S>();
-    __shared__ float lds_b[kTile * NP], lds_c[STATE_ONLY ? 1 : kTile * NP];
+    __shared__ float lds_b[2][kTile * NP], lds_c[STATE_ONLY ? 1 : 2][STATE_ONLY ? 1 : kTile * NP];
     const Place p = place(a, blockIdx.z);
     const int chunk = blockIdx.y, t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.L), tend = min(t1, p.len);
+    const int left = tend - t0;                                       // steps of this chunk
+    Column<T, kTile> xs(a.x, a.xb, a.xt, p, t0), dts(a.dt, a.dtb, a.dtt, p, t0), zs(a.z, a.zb, a.zt, p, t0);
+    Shared<T, S, kTile> bs(a.Bm, a.bb, a.bt, a.bg, p, t0, a.N), cs(a.Cm, a.cb, a.ct, a.cg, p, t0, a.N);
+    auto fetch = [&](int dt) {
+        dts.load(dt, left - dt, p.q);
+        xs.load(dt, left - dt, p.q);
+        if (!STATE_ONLY && a.z) zs.load(dt, left - dt, p.q);
+        bs.load(dt, left - dt);
+        if (!STATE_ONLY) cs.load(dt, left - dt);
+    };
+    if (left > 0) fetch(0);
     float A2[S], h[S];
     load_states<S>(A2, a.A + (size_t)p.ch * a.N, p.q, a.N);
 #pragma unroll
@@ -128,30 +214,37 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
             for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_hw(A2[s] * sd), h[s], e[s]);
         }
     }
+    const OutColumn<T, kTile> out(a.y, a.D, (size_t)p.b * a.L + t0, p);
     float sdt = 0.f;
-    for (int t = t0; t < tend; t += kTile) {
-        __syncthreads();
-        stage_rows<T, S, kTile>(lds_b, a.Bm, p.b * a.bb + p.g * a.bg, a.bt, t, tend, a.N);
-        if (!STATE_ONLY) stage_rows<T, S, kTile>(lds_c, a.Cm, p.b * a.cb + p.g * a.cg, a.ct, t, tend, a.N);
-        __syncthreads();
+    int half = 0;
+    for (int dt0 = 0; dt0 < left; dt0 += kTile, half ^= 1) {
+        float *lb = lds_b[half], *lc = lds_c[STATE_ONLY ? 0 : half];
+        bs.store(lb);
+        if (!STATE_ONLY) cs.store(lc);
+        float x[kTile / 4], dt[kTile / 4], z[kTile / 4], y[kTile / 4];
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i) {
-            if (!STATE_ONLY && a.marks && (4 * i) % MK == 0 && t + 4 * i < tend && p.live)
-                store_padded<S>(h, a.marks + (((size_t)p.b * a.nmark + (t + 4 * i) / MK) * a.D + p.ch) * NP, p.q);
-            const int own = t + 4 * i + p.q;
-            const bool in = own < tend && p.live;
-            float x = 0.f, dt = 0.f;
-            if (in) {
-                x = at<T>(a.x, p.b * a.xb + own * a.xt + p.ch);
-                dt = at<T>(a.dt, p.b * a.dtb + own * a.dtt + p.ch) + bias;
-                if (a.softplus) dt = softplus_exact(dt);
-            }
-            const float u = dt * x;
-            sdt += dt;
+            x[i] = widen(xs.v[i]);
+            dt[i] = widen(dts.v[i]) + bias;
+            z[i] = !STATE_ONLY && a.z ? widen(zs.v[i]) : 0.f;
+        }
+        __syncthreads();
+        if (dt0 + kTile < left) fetch(dt0 + kTile);
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < kTile / 4; ++i) dt[i] = softplus_exact(dt[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kTile / 4; ++i) {
+            if (!STATE_ONLY && a.marks && (4 * i) % MK == 0 && dt0 + 4 * i < left && p.live)
+                store_padded<S>(h, a.marks + (((size_t)p.b * a.nmark + (t0 + dt0 + 4 * i) / MK) * a.D + p.ch) * NP, p.q);
+            dt[i] = dt0 + 4 * i + p.q < left ? dt[i] : 0.f;
+            const float u = dt[i] * x[i];
+            sdt += dt[i];
             float part[4];
             auto step = [&](int j, float dtj, float uj) {
-                const float* bj = lds_b + (4 * i + j) * NP + p.q * S;
-                const float* cj = lds_c + (STATE_ONLY ? 0 : (4 * i + j) * NP + p.q * S);
+                const float* bj = lb + (4 * i + j) * NP + p.q * S;
+                const float* cj = lc + (STATE_ONLY ? 0 : (4 * i + j) * NP + p.q * S);
                 float y = 0.f;
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
@@ -160,20 +253,19 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
                 }
                 part[j] = y;
             };
-            step(0, quad_lane<0>(dt), quad_lane<0>(u));
-            step(1, quad_lane<1>(dt), quad_lane<1>(u));
-            step(2, quad_lane<2>(dt), quad_lane<2>(u));
-            step(3, quad_lane<3>(dt), quad_lane<3>(u));
-            if (!STATE_ONLY) {
-                float y = fmaf(dskip, x, quad_sum_of_own(part[0], part[1], part[2], part[3], p.q));
-                if (in) {
-                    if (a.z) {
-                        const float z = at<T>(a.z, p.b * a.zb + own * a.zt + p.ch);
-                        y *= z * sigmoid_hw(z);
-                    }
-                    static_cast<T*>(a.y)[((size_t)p.b * a.L + own) * a.D + p.ch] = (T)y;
-                }
+            step(0, quad_lane<0>(dt[i]), quad_lane<0>(u));
+            step(1, quad_lane<1>(dt[i]), quad_lane<1>(u));
+            step(2, quad_lane<2>(dt[i]), quad_lane<2>(u));
+            step(3, quad_lane<3>(dt[i]), quad_lane<3>(u));
+            if (!STATE_ONLY) y[i] = fmaf(dskip, x[i], quad_sum_of_own(part[0], part[1], part[2], part[3], p.q));
+        }
+        if (!STATE_ONLY) {
+            if (a.z) {
+#pragma unroll
+                for (int i = 0; i < kTile / 4; ++i) y[i] *= z[i] * sigmoid_hw(z[i]);
             }
+#pragma unroll
+            for (int i = 0; i < kTile / 4; ++i) out.store(dt0, left - dt0, p.q, i, y[i]);
         }
     }
     if (STATE_ONLY) {
@@ -191,48 +283,65 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 }
 
 // The first backward pass over a split time axis: the adjoint that a chunk hands to the chunk before it, from zero,
-// and the sum of its steps.
+// and the sum of its steps.  Built like the forward pass, from the chunk's last tile to its first.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_bwd_state_kernel(ScanArgs a) {
     constexpr int NP = 4 * S;
-    __shared__ float lds_c[kTile * NP];
+    __shared__ float lds_c[2][kTile * NP];
     const Place p = place(a, blockIdx.z);
-    const int chunk = blockIdx.y, t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.L), tend = min(t1, p.len);
+    const int chunk = blockIdx.y + 1;                                 // nobody stands before the first chunk
+    const int t0 = chunk * a.chunk, tend = min(min(t0 + a.chunk, a.L), p.len), left = tend - t0;
+    Column<T, kTile> dys(a.dy, a.dyb, a.dyt, p, t0), dts(a.dt, a.dtb, a.dtt, p, t0), zs(a.z, a.zb, a.zt, p, t0);
+    Shared<T, S, kTile> cs(a.Cm, a.cb, a.ct, a.cg, p, t0, a.N);
+    auto fetch = [&](int dt) {
+        dts.load(dt, left - dt, p.q);
+        dys.load(dt, left - dt, p.q);
+        if (a.z) zs.load(dt, left - dt, p.q);
+        cs.load(dt, left - dt);
+    };
+    int dt0 = left > 0 ? (left - 1) / kTile * kTile : -1;
+    if (dt0 >= 0) fetch(dt0);
     float A2[S], g[S];
     load_states<S>(A2, a.A + (size_t)p.ch * a.N, p.q, a.N);
 #pragma unroll
     for (int s = 0; s < S; ++s) { A2[s] *= kLog2e; g[s] = 0.f; }
     const float bias = a.bias ? a.bias[p.ch] : 0.f;
     float sdt = 0.f;
-    for (int k = (tend - t0 + kTile - 1) / kTile - 1; k >= 0; --k) {
-        const int t = t0 + k * kTile;
+    for (int half = 0; dt0 >= 0; dt0 -= kTile, half ^= 1) {
+        float* lc = lds_c[half];
+        cs.store(lc);
+        float dt[kTile / 4], dy[kTile / 4], z[kTile / 4];
+#pragma unroll
+        for (int i = 0; i < kTile / 4; ++i) {
+            dt[i] = widen(dts.v[i]) + bias;
+            dy[i] = widen(dys.v[i]);
+            z[i] = a.z ? widen(zs.v[i]) : 0.f;
+        }
         __syncthreads();
-        stage_rows<T, S, kTile>(lds_c, a.Cm, p.b * a.cb + p.g * a.cg, a.ct, t, tend, a.N);
-        __syncthreads();
+        if (dt0 > 0) fetch(dt0 - kTile);
+        if (a.softplus) {
+#pragma unroll
+            for (int i = 0; i < kTile / 4; ++i) dt[i] = softplus_exact(dt[i]);
+        }
+        if (a.z) {
+#pragma unroll
+            for (int i = 0; i < kTile / 4; ++i) dy[i] *= z[i] * sigmoid_hw(z[i]);
+        }
 #pragma unroll
         for (int i = kTile / 4 - 1; i >= 0; --i) {
-            const int own = t + 4 * i + p.q;
-            const bool in = own < tend && p.live;
-            float dt = 0.f, dy = 0.f;
-            if (in) {
-                dt = at<T>(a.dt, p.b * a.dtb + own * a.dtt + p.ch) + bias;
-                if (a.softplus) dt = softplus_exact(dt);
-                dy = at<T>(a.dy, p.b * a.dyb + own * a.dyt + p.ch);
-                if (a.z) {
-                    const float z = at<T>(a.z, p.b * a.zb + own * a.zt + p.ch);
-                    dy *= z * sigmoid_hw(z);
-                }
-            }
-            sdt += dt;
+            const bool in = dt0 + 4 * i + p.q < left;
+            dt[i] = in ? dt[i] : 0.f;
+            dy[i] = in ? dy[i] : 0.f;
+            sdt += dt[i];
             auto step = [&](int j, float dtj, float dyj) {
-                const float* cj = lds_c + (4 * i + j) * NP + p.q * S;
+                const float* cj = lc + (4 * i + j) * NP + p.q * S;
 #pragma unroll
                 for (int s = 0; s < S; ++s) g[s] = exp2_hw(A2[s] * dtj) * fmaf(dyj, cj[s], g[s]);
             };
-            step(3, quad_lane<3>(dt), quad_lane<3>(dy));
-            step(2, quad_lane<2>(dt), quad_lane<2>(dy));
-            step(1, quad_lane<1>(dt), quad_lane<1>(dy));
-            step(0, quad_lane<0>(dt), quad_lane<0>(dy));
+            step(3, quad_lane<3>(dt[i]), quad_lane<3>(dy[i]));
+            step(2, quad_lane<2>(dt[i]), quad_lane<2>(dy[i]));
+            step(1, quad_lane<1>(dt[i]), quad_lane<1>(dy[i]));
+            step(0, quad_lane<0>(dt[i]), quad_lane<0>(dy[i]));
         }
     }
     const size_t row = ((size_t)p.b * a.nchunk + chunk) * a.D + p.ch;
@@ -243,12 +352,43 @@ __global__ __launch_bounds__(256) void scan_bwd_state_kernel(ScanArgs a) {
     }
 }
 
-// sum over the 16 channels of a wave (lanes of one place in their quads); every lane gets it
-__device__ __forceinline__ float channel_sum(float v) {
-    v += dpp<0x124>(v);                   // row_ror:4
-    v += dpp<0x128>(v);                   // row_ror:8
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+// Sums over the 16 channels of a wave of v[m][s], m = 0..MK-1 steps: an exchange of lane halves sums two steps at a time
+// (each half of the lanes keeps one of them), then of rows of 16 lanes, then the four quads of a row are summed in place.
+// Afterwards v[m][s], m < MK/4, holds the sums of step m + MK/4 * r in row r of lanes.
+template <int MK, int S>
+__device__ __forceinline__ void channel_sums(float (&v)[MK][S]) {
+    constexpr int H = MK / 2, Q = MK / 4;
+#pragma unroll
+    for (int e = 0; e < H * S; e += 4) {
+        float *a[4], *b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = &v[(e + k) / S][(e + k) % S];
+            b[k] = &v[(e + k) / S + H][(e + k) % S];
+        }
+        swap32(*a[0], *b[0], *a[1], *b[1], *a[2], *b[2], *a[3], *b[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *a[k] += *b[k];
+    }
+#pragma unroll
+    for (int e = 0; e < Q * S; e += 4) {
+        float *a[4], *b[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            a[k] = &v[(e + k) / S][(e + k) % S];
+            b[k] = &v[(e + k) / S + Q][(e + k) % S];
+        }
+        swap16(*a[0], *b[0], *a[1], *b[1], *a[2], *b[2], *a[3], *b[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *a[k] += *b[k];
+    }
+#pragma unroll
+    for (int m = 0; m < Q; ++m)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            v[m][s] += dpp<0x128>(v[m][s]);           // row_ror:8
+            v[m][s] += dpp<0x124>(v[m][s]);           // row_ror:4
+        }
 }
 
 // Backward on a chunk, tile after tile from its end.  A tile's states are computed again from the state saved in front
@@ -256,13 +396,31 @@ __device__ __forceinline__ float channel_sum(float v) {
 //     g_t = C_t dy'_t + a_{t+1} g_{t+1},  dy' = dy silu(z)
 //     dC_t = sum_d dy' h_t,  dB_t = sum_d g_t u_t,  du = g_t . B_t,  w = g_t a_t h_{t-1}
 //     d raw = (A . w + du x) sigmoid(raw),  dx = du dt + D dy',  dA = sum w dt
+// A channel's shares of dB and dC take the registers of its a_t and h_t; they are summed over the wave by lane exchanges
+// and over the block's waves through LDS, and the block writes one row of partial sums per step.  One barrier a tile: the
+// LDS areas are used in turn, and a tile's sums are taken after the next one's barrier.
 template <class T, int S>
-__global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs a) {
-    constexpr int NP = 4 * S, MK = mark_steps<S>(), NI = MK / 4;
-    __shared__ float lds_b[MK * NP], lds_c[MK * NP], red[4 * MK * 2 * NP];       // red: [wave][step][B, C][state]
+__global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs a) {
+    constexpr int NP = 4 * S, MK = mark_steps<S>(), NI = MK / 4, RED = MK * 2 * NP;
+    __shared__ float lds_b[2][MK * NP], lds_c[2][MK * NP];
+    __shared__ __attribute__((aligned(16))) float red[2][4 * RED];    // [wave][step][B, C][state]
     const Place p = place(a, blockIdx.z);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int chunk = blockIdx.y, t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.L), tend = min(t1, p.len);
+    const int chunk = blockIdx.y, t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.L), tend = min(t1, p.len), left = tend - t0;
+    Column<T, MK> xs(a.x, a.xb, a.xt, p, t0), dts(a.dt, a.dtb, a.dtt, p, t0), zs(a.z, a.zb, a.zt, p, t0), dys(a.dy, a.dyb, a.dyt, p, t0);
+    Shared<T, S, MK> bs(a.Bm, a.bb, a.bt, a.bg, p, t0, a.N), cs(a.Cm, a.cb, a.ct, a.cg, p, t0, a.N);
+    float h0[S];
+    auto fetch = [&](int dt) {
+        dts.load(dt, left - dt, p.q);
+        xs.load(dt, left - dt, p.q);
+        dys.load(dt, left - dt, p.q);
+        if (a.z) zs.load(dt, left - dt, p.q);
+        bs.load(dt, left - dt);
+        cs.load(dt, left - dt);
+        load_padded<S>(h0, a.marks + ((size_t)p.b * a.nmark + (t0 + dt) / MK) * a.D * NP + (unsigned)p.ch * NP, p.q);
+    };
+    int dt0 = left > 0 ? (left - 1) / MK * MK : -1;
+    if (dt0 >= 0) fetch(dt0);
     float A2[S], g[S], dA[S];
     load_states<S>(A2, a.A + (size_t)p.ch * a.N, p.q, a.N);
 #pragma unroll
@@ -277,71 +435,89 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
         for (int s = 0; s < S; ++s) g[s] = fmaf(exp2_hw(A2[s] * sd), g[s], e[s]);
     }
+    const size_t first = (size_t)p.b * a.L + t0;                      // row of the chunk's first step
+    const OutColumn<T, MK> dx(a.dx, a.D, first, p), ddt(a.ddt, a.D, first, p), dz(a.dz, a.D, first, p);
+    auto write_sums = [&](int dt, const float* r) {                   // of the tile at dt
+        float* dst = a.pBC + ((first + dt) * gridDim.x + blockIdx.x) * (2 * NP);
+        for (int e = threadIdx.x; e < RED; e += 256)
+            if (dt + e / (2 * NP) < left)
+                dst[(size_t)(e / (2 * NP)) * gridDim.x * (2 * NP) + e % (2 * NP)] = (r[e] + r[e + RED]) + (r[e + 2 * RED] + r[e + 3 * RED]);
+    };
     float dD = 0.f, dbias = 0.f;
-    for (int k = (tend - t0 + MK - 1) / MK - 1; k >= 0; --k) {
-        const int t = t0 + k * MK;
-        __syncthreads();
-        stage_rows<T, S, MK>(lds_b, a.Bm, p.b * a.bb + p.g * a.bg, a.bt, t, tend, a.N);
-        stage_rows<T, S, MK>(lds_c, a.Cm, p.b * a.cb + p.g * a.cg, a.ct, t, tend, a.N);
-        float h0[S];
-        load_padded<S>(h0, a.marks + (((size_t)p.b * a.nmark + t / MK) * a.D + p.ch) * NP, p.q);
-        float raw[NI], dt[NI], u[NI], x[NI], dy[NI];
+    int half = 0, before = -1;                                        // before: the tile whose sums wait in the other half
+    for (; dt0 >= 0; dt0 -= MK, half ^= 1) {
+        float *lb = lds_b[half], *lc = lds_c[half];
+        bs.store(lb);
+        cs.store(lc);
+        float sg[NI], dt[NI], x[NI], dy[NI], z[NI], h1[S];
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-            const int own = t + 4 * i + p.q;
-            const bool in = own < tend && p.live;
-            raw[i] = dt[i] = x[i] = dy[i] = 0.f;
-            if (in) {
-                x[i] = at<T>(a.x, p.b * a.xb + own * a.xt + p.ch);
-                raw[i] = at<T>(a.dt, p.b * a.dtb + own * a.dtt + p.ch) + bias;
-                dt[i] = a.softplus ? softplus_exact(raw[i]) : raw[i];
-                dy[i] = at<T>(a.dy, p.b * a.dyb + own * a.dyt + p.ch);
-            }
-            u[i] = dt[i] * x[i];
+            x[i] = widen(xs.v[i]);
+            dt[i] = widen(dts.v[i]) + bias;
+            dy[i] = widen(dys.v[i]);
+            z[i] = a.z ? widen(zs.v[i]) : 0.f;
         }
+#pragma unroll
+        for (int s = 0; s < S; ++s) h1[s] = h0[s];
         __syncthreads();
-        float av[MK][S], h[MK][S];
+        if (before >= 0) write_sums(before, red[half ^ 1]);
+        before = dt0;
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
+            const bool in = dt0 + 4 * i + p.q < left && p.live;
+            sg[i] = a.softplus ? sigmoid_hw(dt[i]) : 1.f;
+            if (a.softplus) dt[i] = softplus_exact(dt[i]);
+            dt[i] = in ? dt[i] : 0.f;
+            x[i] = in ? x[i] : 0.f;
+            dy[i] = in ? dy[i] : 0.f;
+        }
+        float av[MK][S], h[MK][S], y[NI];
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
             float part[4];
+            const float u = dt[i] * x[i];
             auto step = [&](int j, float dtj, float uj) {
                 const int m = 4 * i + j;
-                const float *bj = lds_b + m * NP + p.q * S, *cj = lds_c + m * NP + p.q * S;
-                float y = 0.f;
+                const float *bj = lb + m * NP + p.q * S, *cj = lc + m * NP + p.q * S;
+                float yj = 0.f;
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     av[m][s] = exp2_hw(A2[s] * dtj);
-                    h[m][s] = fmaf(av[m][s], m ? h[m - 1][s] : h0[s], uj * bj[s]);
-                    y = fmaf(h[m][s], cj[s], y);
+                    h[m][s] = fmaf(av[m][s], m ? h[m - 1][s] : h1[s], uj * bj[s]);
+                    yj = fmaf(h[m][s], cj[s], yj);
                 }
-                part[j] = y;
+                part[j] = yj;
             };
-            step(0, quad_lane<0>(dt[i]), quad_lane<0>(u[i]));
-            step(1, quad_lane<1>(dt[i]), quad_lane<1>(u[i]));
-            step(2, quad_lane<2>(dt[i]), quad_lane<2>(u[i]));
-            step(3, quad_lane<3>(dt[i]), quad_lane<3>(u[i]));
-            if (a.z) {
-                const float y = fmaf(dskip, x[i], quad_sum_of_own(part[0], part[1], part[2], part[3], p.q));
-                const int own = t + 4 * i + p.q;
-                if (own < tend && p.live) {
-                    const float z = at<T>(a.z, p.b * a.zb + own * a.zt + p.ch), sg = sigmoid_hw(z);
-                    static_cast<T*>(a.dz)[((size_t)p.b * a.L + own) * a.D + p.ch] = (T)(dy[i] * y * sg * fmaf(z, 1.f - sg, 1.f));
-                    dy[i] *= z * sg;
-                }
+            step(0, quad_lane<0>(dt[i]), quad_lane<0>(u));
+            step(1, quad_lane<1>(dt[i]), quad_lane<1>(u));
+            step(2, quad_lane<2>(dt[i]), quad_lane<2>(u));
+            step(3, quad_lane<3>(dt[i]), quad_lane<3>(u));
+            y[i] = fmaf(dskip, x[i], quad_sum_of_own(part[0], part[1], part[2], part[3], p.q));
+        }
+        if (a.z) {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const float s = sigmoid_hw(z[i]);
+                dz.store(dt0, left - dt0, p.q, i, dy[i] * y[i] * s * fmaf(z[i], 1.f - s, 1.f));
+                dy[i] *= z[i] * s;
             }
         }
+        if (dt0 > 0) fetch(dt0 - MK);
 #pragma unroll
         for (int i = NI - 1; i >= 0; --i) {
+            __builtin_amdgcn_sched_barrier(0);
             float pu[4], pt[4];
+            const float u = dt[i] * x[i];
             auto step = [&](int j, float dtj, float uj, float dyj) {
                 const int m = 4 * i + j;
-                const float *bj = lds_b + m * NP + p.q * S, *cj = lds_c + m * NP + p.q * S;
+                const float *bj = lb + m * NP + p.q * S, *cj = lc + m * NP + p.q * S;
                 float du = 0.f, dd = 0.f;
 #pragma unroll
                 for (int s = 0; s < S; ++s) {
                     g[s] = fmaf(dyj, cj[s], g[s]);
                     du = fmaf(g[s], bj[s], du);
-                    const float ga = g[s] * av[m][s], w = ga * (m ? h[m - 1][s] : h0[s]);
+                    const float ga = g[s] * av[m][s], w = ga * (m ? h[m - 1][s] : h1[s]);
                     dd = fmaf(A2[s], w, dd);
                     dA[s] = fmaf(dtj, w, dA[s]);
                     av[m][s] = g[s] * uj;                 // dB of this channel
@@ -351,49 +527,43 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanArgs a) {
                 pu[j] = du;
                 pt[j] = dd;
             };
-            step(3, quad_lane<3>(dt[i]), quad_lane<3>(u[i]), quad_lane<3>(dy[i]));
-            step(2, quad_lane<2>(dt[i]), quad_lane<2>(u[i]), quad_lane<2>(dy[i]));
-            step(1, quad_lane<1>(dt[i]), quad_lane<1>(u[i]), quad_lane<1>(dy[i]));
-            step(0, quad_lane<0>(dt[i]), quad_lane<0>(u[i]), quad_lane<0>(dy[i]));
+            step(3, quad_lane<3>(dt[i]), quad_lane<3>(u), quad_lane<3>(dy[i]));
+            step(2, quad_lane<2>(dt[i]), quad_lane<2>(u), quad_lane<2>(dy[i]));
+            step(1, quad_lane<1>(dt[i]), quad_lane<1>(u), quad_lane<1>(dy[i]));
+            step(0, quad_lane<0>(dt[i]), quad_lane<0>(u), quad_lane<0>(dy[i]));
             const float du = quad_sum_of_own(pu[0], pu[1], pu[2], pu[3], p.q);
-            float dr = kLn2 * quad_sum_of_own(pt[0], pt[1], pt[2], pt[3], p.q) + du * x[i];
-            if (a.softplus) dr *= sigmoid_hw(raw[i]);
-            const int own = t + 4 * i + p.q;
-            if (own < tend && p.live) {
-                const size_t o = ((size_t)p.b * a.L + own) * a.D + p.ch;
-                static_cast<T*>(a.dx)[o] = (T)fmaf(du, dt[i], dskip * dy[i]);
-                static_cast<T*>(a.ddt)[o] = (T)dr;
-                dbias += dr;
-                dD = fmaf(dy[i], x[i], dD);
-            }
+            const float dr = sg[i] * fmaf(kLn2, quad_sum_of_own(pt[0], pt[1], pt[2], pt[3], p.q), du * x[i]);
+            dx.store(dt0, left - dt0, p.q, i, fmaf(du, dt[i], dskip * dy[i]));
+            ddt.store(dt0, left - dt0, p.q, i, dr);
+            dbias += dt0 + 4 * i + p.q < left ? dr : 0.f;
+            dD = fmaf(dy[i], x[i], dD);
         }
+        channel_sums<MK, S>(av);
+        channel_sums<MK, S>(h);
+        if ((lane & 12) == 0) {
+            const int m0 = (lane >> 4) * (MK / 4);
+            float* r = red[half] + (wave * MK + m0) * 2 * NP + p.q * S;
 #pragma unroll
-        for (int m = 0; m < MK; ++m)
+            for (int m = 0; m < MK / 4; ++m) {
+                Pack<float, S> vb, vc;
 #pragma unroll
-            for (int s = 0; s < S; ++s) {
-                const float vb = channel_sum(av[m][s]), vc = channel_sum(h[m][s]);
-                if (lane < 4) {
-                    float* r = red + (wave * MK + m) * 2 * NP + p.q * S + s;
-                    r[0] = vb;
-                    r[NP] = vc;
-                }
+                for (int s = 0; s < S; ++s) { vb.set(s, av[m][s]); vc.set(s, h[m][s]); }
+                vb.store(r + m * 2 * NP);
+                vc.store(r + m * 2 * NP + NP);
             }
-        __syncthreads();
-        for (int e = threadIdx.x; e < MK * 2 * NP; e += 256) {
-            const int m = e / (2 * NP), r = e % (2 * NP);
-            if (t + m < tend)
-                a.pBC[(((size_t)p.b * a.L + t + m) * gridDim.x + blockIdx.x) * 2 * NP + r] =
-                    (red[e] + red[e + MK * 2 * NP]) + (red[e + 2 * MK * 2 * NP] + red[e + 3 * MK * 2 * NP]);
         }
     }
+    __syncthreads();
+    if (before >= 0) write_sums(before, red[half ^ 1]);
     dD = quad_sum(dD);
     dbias = quad_sum(dbias);
     if (!p.live) return;
-    const size_t part = (size_t)p.b * a.nchunk + chunk;
-    store_padded<S>(dA, a.pA + (part * a.D + p.ch) * NP, p.q);
+    float* part = a.pA + ((size_t)p.b * a.nchunk + chunk) * a.D * (NP + 2);
+#pragma unroll
+    for (int s = 0; s < S; ++s) part[(size_t)p.ch * NP + p.q * S + s] = dA[s];
     if (p.q == 0) {
-        a.pD[(part * 2 + 0) * a.D + p.ch] = dD;
-        a.pD[(part * 2 + 1) * a.D + p.ch] = dbias;
+        part[(size_t)a.D * NP + p.ch] = dD;
+        part[(size_t)a.D * (NP + 1) + p.ch] = dbias;
     }
     if (chunk == 0 && a.dh0) store_states<S>(g, a.dh0 + ((size_t)p.b * a.D + p.ch) * a.N, p.q, a.N);
     for (int t = max(t0, tend) + p.q; t < t1; t += 4) {                // behind the sequence's end
@@ -421,57 +591,56 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
     (r < NP ? dB : dC)[row * N + n] = (T)s;
 }
 
-// rows of NP with N used -> [D, N], summed over R partials
-__global__ __launch_bounds__(256) void scan_dA_kernel(const float* __restrict__ part, float* __restrict__ dA, int R, int D, int N, int NP) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= D * N) return;
-    const int d = i / N, n = i - d * N;
-    float s = 0.f;
-    for (int r = 0; r < R; ++r) s += part[((size_t)r * D + d) * NP + n];
-    dA[i] = s;
-}
-
-// One token of every row; state [slots, D, N] is read and written once: 8N bytes a channel against 7N operations.
+// One token of every row; state [slots, D, N] is read and written once: 8N bytes a channel against 7N operations, HBM
+// bound.  A block takes a row's blocks of 64 channels in turn (of one group: B and C are loaded once), so that the check of
+// the row's slot against the rows before it is paid once for several of them.
 template <class T, int S>
-__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, const int* __restrict__ slots, int nslots, float* __restrict__ state) {
-    const int row = blockIdx.y;
+__global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, int parts, const int* __restrict__ slots, int nslots, float* __restrict__ state) {
+    const int row = blockIdx.y, g = blockIdx.x / parts, part = blockIdx.x - g * parts;
+    const int q = threadIdx.x & 3, lane_ch = threadIdx.x >> 2;
+    const bool whole = a.N == 4 * S;                                  // a lane's states are one vector
+    float B[S], C[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int n = q * S + s;
+        B[s] = n < a.N ? at<T>(a.Bm, row * a.bb + g * a.bg + n) : 0.f;
+        C[s] = n < a.N ? at<T>(a.Cm, row * a.cb + g * a.cg + n) : 0.f;
+    }
     bool bad;
     const int slot = claim_slot(slots, row, nslots, &bad);
-    const Place p = place(a, row);
-    if (!p.live) return;
-    T* out = static_cast<T*>(a.y) + (size_t)row * a.D + p.ch;
-    if (bad || slot < 0) {
-        if (p.q == 0) *out = (T)(bad ? __builtin_nanf("") : 0.f);
-        return;
-    }
-    float* st = state + ((size_t)slot * a.D + p.ch) * a.N;
-    float h[S], A2[S], B[S], C[S];
-    load_states<S>(h, st, p.q, a.N);
-    load_states<S>(A2, a.A + (size_t)p.ch * a.N, p.q, a.N);
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        const int n = p.q * S + s;
-        B[s] = n < a.N ? at<T>(a.Bm, row * a.bb + p.g * a.bg + n) : 0.f;
-        C[s] = n < a.N ? at<T>(a.Cm, row * a.cb + p.g * a.cg + n) : 0.f;
-    }
-    const float x = at<T>(a.x, row * a.xb + p.ch);
-    float dt = at<T>(a.dt, row * a.dtb + p.ch) + (a.bias ? a.bias[p.ch] : 0.f);
-    if (a.softplus) dt = softplus_exact(dt);
-    float y = 0.f;
-#pragma unroll
-    for (int s = 0; s < S; ++s) {
-        h[s] = fmaf(exp2_hw(A2[s] * kLog2e * dt), h[s], dt * x * B[s]);
-        y = fmaf(h[s], C[s], y);
-    }
-    store_states<S>(h, st, p.q, a.N);
-    y = quad_sum(y);
-    if (p.q == 0) {
-        if (a.Dp) y = fmaf(a.Dp[p.ch], x, y);
-        if (a.z) {
-            const float z = at<T>(a.z, row * a.zb + p.ch);
-            y *= z * sigmoid_hw(z);
+    for (int tile = part; tile < a.tpg; tile += parts) {
+        if (tile * kCh + lane_ch >= a.Dg) break;
+        const int ch = g * a.Dg + tile * kCh + lane_ch;
+        T* out = static_cast<T*>(a.y) + (size_t)row * a.D + ch;
+        if (bad || slot < 0) {
+            if (q == 0) *out = (T)(bad ? __builtin_nanf("") : 0.f);
+            continue;
         }
-        *out = (T)y;
+        float* st = state + ((size_t)slot * a.D + ch) * a.N;
+        const float* Ap = a.A + (size_t)ch * a.N;
+        float h[S], A2[S];
+        if (whole) {
+            load_padded<S>(h, st, q);
+            load_padded<S>(A2, Ap, q);
+        } else {
+            load_states<S>(h, st, q, a.N);
+            load_states<S>(A2, Ap, q, a.N);
+        }
+        const float x = at<T>(a.x, row * a.xb + ch), z = a.z ? at<T>(a.z, row * a.zb + ch) : 0.f;
+        float dt = at<T>(a.dt, row * a.dtb + ch) + (a.bias ? a.bias[ch] : 0.f);
+        if (a.softplus) dt = softplus_exact(dt);
+        float y = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            h[s] = fmaf(exp2_hw(A2[s] * kLog2e * dt), h[s], dt * x * B[s]);
+            y = fmaf(h[s], C[s], y);
+        }
+        if (whole) store_padded<S>(h, st, q);
+        else store_states<S>(h, st, q, a.N);
+        y = quad_sum(y);
+        if (a.Dp) y = fmaf(a.Dp[ch], x, y);
+        if (a.z) y *= z * sigmoid_hw(z);
+        if (q == 0) *out = (T)y;
     }
 }
 
@@ -483,16 +652,21 @@ struct ScanPlan {
     int S, NP, tpg, nchunk, chunk, nmark;
 };
 
-// Time is split where the channels of the batch alone do not fill the chip.
-ScanPlan scan_plan(const UnetmiScanDesc& d) {
+// Time is split where the blocks of the batch's channels alone do not fill the chip's 256 CUs: the first pass over the
+// chunks costs about 0.6 of the second, so it does not pay before (128 sequences of 501 steps, 512 blocks: 104 us in one
+// chunk, 35 + 94 us in two; 1 x 8192 steps x 2048 channels, 32 blocks: 99 + 64 us in 16 chunks, 90 + 60 in 32, 98 + 58 in
+// 64).  The backward kernel, two blocks a CU, gains from a split up to 384.  Sequences that end early (`ragged`) leave
+// their last chunks empty, and finer chunks even that out (8 x 2001 x 1280: 195 us in 3 chunks, 156 in 6, 122 in 21).
+ScanPlan scan_plan(const UnetmiScanDesc& d, bool ragged, bool backward) {
     ScanPlan p;
     p.S = lane_states(d.state);
     p.NP = 4 * p.S;
     const int Dg = d.channels / d.groups;
     p.tpg = (Dg + kCh - 1) / kCh;
     const long long blocks = (long long)d.batch * d.groups * p.tpg;
-    long long want = blocks > 0 ? 512 / blocks : 1;
-    const long long most = (d.length + 63) / 64;
+    long long want = 1;
+    if (blocks > 0 && blocks < (backward ? 384 : 256)) want = ((ragged ? 4096 : 1024) + blocks - 1) / blocks;
+    const long long most = (d.length + 63) / 64;                      // chunks of at least 64 steps
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
@@ -514,11 +688,15 @@ int scan_check(const UnetmiScanDesc* d, const char* what) {
     if (d->state > 64) return api_fail(UNETMI_E_UNSUPPORTED, w + ": at most 64 states per channel are built");
     if (d->dtype != UNETMI_DTYPE_F32 && d->dtype != UNETMI_DTYPE_BF16) return api_fail(UNETMI_E_UNSUPPORTED, w + ": fp32 or bfloat16 activations");
     if (d->batch > 65535) return api_fail(UNETMI_E_UNSUPPORTED, w + ": more than 65535 sequences");
-    if (d->channels > (1 << 24) || d->length > (1 << 28)) return api_fail(UNETMI_E_UNSUPPORTED, w + ": more than 2^24 channels or 2^28 steps");
-    for (const int64_t* s : {d->x_stride, d->dt_stride, d->z_stride, d->dy_stride})
+    if (d->channels > (1 << 22) || d->length > (1 << 28)) return api_fail(UNETMI_E_UNSUPPORTED, w + ": more than 2^22 channels or 2^28 steps");
+    for (const int64_t* s : {d->x_stride, d->dt_stride, d->z_stride, d->dy_stride}) {
         if (s[0] < 0 || s[1] < 0) return api_fail(UNETMI_E_BAD_DESC, w + ": negative stride");
+        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^25 elements apart");
+    }
     for (const int64_t* s : {d->b_stride, d->c_stride})
         if (s[0] < 0 || s[1] < 0 || s[2] < 0) return api_fail(UNETMI_E_BAD_DESC, w + ": negative stride");
+    for (const int64_t* s : {d->b_stride, d->c_stride})
+        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^25 elements apart");
     return UNETMI_OK;
 }
 
@@ -570,7 +748,7 @@ struct RunScanBwd {
         const dim3 block(256), grid(d.groups * p.tpg, p.nchunk, d.batch);
         int rc;
         if (p.nchunk > 1) {
-            hipLaunchKernelGGL((scan_bwd_state_kernel<T, S>), grid, block, 0, s, a);
+            hipLaunchKernelGGL((scan_bwd_state_kernel<T, S>), dim3(d.groups * p.tpg, p.nchunk - 1, d.batch), block, 0, s, a);
             if ((rc = launched("ssm_scan_bwd states")) != UNETMI_OK) return rc;
         }
         hipLaunchKernelGGL((scan_bwd_kernel<T, S>), grid, block, 0, s, a);
@@ -581,16 +759,17 @@ struct RunScanBwd {
                                static_cast<T*>(dC), a.lengths, rows, d.length, d.groups, p.tpg, d.state, p.NP);
             if ((rc = launched("ssm_scan_bwd B C")) != UNETMI_OK) return rc;
         }
-        const int parts = d.batch * p.nchunk;
-        hipLaunchKernelGGL(scan_dA_kernel, dim3((d.channels * d.state + 255) / 256), block, 0, s, a.pA, dA, parts, d.channels, d.state, p.NP);
-        if ((rc = launched("ssm_scan_bwd A")) != UNETMI_OK) return rc;
-        return launch_sum_rows(a.pD, dD, dbias, d.channels, parts, 2 * d.channels, s);
+        return launch_sum_rows(a.pA, d.batch * p.nchunk, {dA, d.channels * p.NP, p.NP, d.state}, {dD, d.channels, 1, 1},
+                               {dbias, d.channels, 1, 1}, s);
     }
 };
 template <class T, int S>
 struct RunScanStep {
     static int run(const UnetmiScanDesc& d, const ScanPlan& p, const ScanArgs& a, const int* slots, int nslots, float* state, hipStream_t s) {
-        hipLaunchKernelGGL((scan_step_kernel<T, S>), dim3(d.groups * p.tpg, d.batch), dim3(256), 0, s, a, slots, nslots, state);
+        // about four blocks a CU, as long as that many rows and channels are there
+        long long parts = (1024 + (long long)d.batch * d.groups - 1) / ((long long)d.batch * d.groups);
+        if (parts > p.tpg) parts = p.tpg;
+        hipLaunchKernelGGL((scan_step_kernel<T, S>), dim3(d.groups * (int)parts, d.batch), dim3(256), 0, s, a, (int)parts, slots, nslots, state);
         return launched("ssm_scan_step");
     }
 };
@@ -608,13 +787,13 @@ extern "C" {
 
 size_t unetmi_ssm_scan_marks_bytes(const UnetmiScanDesc* d) {
     if (scan_check(d, "ssm_scan_marks_bytes") != UNETMI_OK) return 0;
-    const ScanPlan p = scan_plan(*d);
+    const ScanPlan p = scan_plan(*d, false, false);
     return (size_t)d->batch * p.nmark * d->channels * p.NP * sizeof(float);
 }
 
-size_t unetmi_ssm_scan_fwd_workspace_bytes(const UnetmiScanDesc* d) {
+size_t unetmi_ssm_scan_fwd_workspace_bytes(const UnetmiScanDesc* d, int ragged) {
     if (scan_check(d, "ssm_scan_fwd_workspace_bytes") != UNETMI_OK) return 0;
-    return summary_floats(*d, scan_plan(*d)) * sizeof(float);
+    return summary_floats(*d, scan_plan(*d, ragged != 0, false)) * sizeof(float);
 }
 
 int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
@@ -624,7 +803,7 @@ int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
     if (rc != UNETMI_OK) return rc;
     if (d->batch == 0 || (d->length == 0 && !state_out)) return UNETMI_OK;
     if (!A || (d->length > 0 && (!x || !dt || !B || !C || !y))) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_fwd: null tensor pointer");
-    const ScanPlan p = scan_plan(*d);
+    const ScanPlan p = scan_plan(*d, lengths != nullptr, false);
     const size_t need = summary_floats(*d, p);
     if (need && (!ws || ws_bytes < need * sizeof(float))) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_fwd: workspace too small");
     ScanArgs a = scan_args(*d, p, x, dt, A, B, C, D, z, dt_bias);
@@ -634,9 +813,9 @@ int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
     return scan_dispatch<RunScan>(*d, p.S, *d, p, a, static_cast<hipStream_t>(stream));
 }
 
-size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d) {
+size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d, int ragged) {
     if (scan_check(d, "ssm_scan_bwd_workspace_bytes") != UNETMI_OK) return 0;
-    const ScanPlan p = scan_plan(*d);
+    const ScanPlan p = scan_plan(*d, ragged != 0, true);
     const size_t parts = (size_t)d->batch * p.nchunk;
     return (summary_floats(*d, p) + (size_t)d->batch * d->length * d->groups * p.tpg * 2 * p.NP + parts * d->channels * (p.NP + 2)) * sizeof(float);
 }
@@ -651,17 +830,16 @@ int unetmi_ssm_scan_bwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
     if (!A || !dA || !dD || !ddt_bias || !ws || (d->length > 0 && (!x || !dt || !B || !C || !marks || !dy || !dx || !ddt || !dB || !dC)))
         return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_bwd: null tensor pointer");
     if (d->length > 0 && (z != nullptr) != (dz != nullptr)) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_bwd: z and dz go together");
-    if (ws_bytes < unetmi_ssm_scan_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_bwd: workspace too small");
-    const ScanPlan p = scan_plan(*d);
+    if (ws_bytes < unetmi_ssm_scan_bwd_workspace_bytes(d, lengths != nullptr)) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_bwd: workspace too small");
+    const ScanPlan p = scan_plan(*d, lengths != nullptr, true);
     ScanArgs a = scan_args(*d, p, x, dt, A, B, C, D, z, dt_bias);
     a.lengths = lengths; a.marks = const_cast<float*>(marks);
     a.dy = dy; a.dhT = dstate_out; a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dstate;
     const size_t parts = (size_t)d->batch * p.nchunk;
-    a.pA = static_cast<float*>(ws);                                   // padded rows first: they stay 16-byte aligned
-    a.pBC = a.pA + parts * d->channels * p.NP;
-    a.hend = a.pBC + (size_t)d->batch * d->length * d->groups * p.tpg * 2 * p.NP;
-    a.sdt = a.hend + (p.nchunk > 1 ? parts * d->channels * p.NP : 0);
-    a.pD = a.sdt + (p.nchunk > 1 ? parts * d->channels : 0);
+    a.hend = static_cast<float*>(ws);                                 // multiples of four floats first: they stay 16-byte aligned
+    a.pBC = a.hend + (p.nchunk > 1 ? parts * d->channels * p.NP : 0);
+    a.pA = a.pBC + (size_t)d->batch * d->length * d->groups * p.tpg * 2 * p.NP;
+    a.sdt = a.pA + parts * d->channels * (p.NP + 2);
     return scan_dispatch<RunScanBwd>(*d, p.S, *d, p, a, dB, dC, dA, dD, ddt_bias, static_cast<hipStream_t>(stream));
 }
 
@@ -673,7 +851,7 @@ int unetmi_ssm_scan_step(const UnetmiScanDesc* d, const void* x, const void* dt,
     if (d->batch == 0) return UNETMI_OK;
     if (!x || !dt || !A || !B || !C || !state || !y) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_step: null tensor pointer");
     if (num_slots < 0 || (!slots && num_slots < d->batch)) return api_fail(UNETMI_E_BAD_ARG, "ssm_scan_step: fewer slots than rows");
-    const ScanPlan p = scan_plan(*d);
+    const ScanPlan p = scan_plan(*d, false, false);
     ScanArgs a = scan_args(*d, p, x, dt, A, B, C, D, z, dt_bias);
     a.y = y;
     return scan_dispatch<RunScanStep>(*d, p.S, *d, p, a, slots, num_slots, state, static_cast<hipStream_t>(stream));

@@ -35,8 +35,9 @@ class _BlockNorm(torch.autograd.Function):
         has = ctx.residual is not None
         dx, dgate, dres, dw = _ops.block_norm_bwd(x, gate, post_weight, stream, scale, pre_weight, ctx.eps, d_out, d_norm, has,
                                                   has and ctx.residual == torch.float32)
-        grads = (dx, None if gate is None else dgate, None if post_weight is None else dw[0], dres if has else None,
-                 None if scale is None else dw[1], None if pre_weight is None else dw[2])
+        d_post, d_scale, d_pre = dw.unbind()
+        grads = (dx, None if gate is None else dgate, None if post_weight is None else d_post, dres if has else None,
+                 None if scale is None else d_scale, None if pre_weight is None else d_pre)
         return tuple(g if n else None for g, n in zip(grads, ctx.needs_input_grad)) + (None,)
 
 
@@ -62,9 +63,7 @@ def block_norm(x, gate=None, post_weight=None, residual=None, scale=None, pre_we
 
 
 def _flat(t, shape):
-    """[..., channels] as rows; a copy only where the rows are not evenly spaced or not dense."""
+    """[..., channels] as rows; a copy only where the rows are not evenly spaced."""
     if t.shape != shape:
         raise ValueError("unet_amd.norm: x, gate and residual have one shape, got {} and {}".format(tuple(shape), tuple(t.shape)))
-    if t.stride(-1) != 1 and shape[-1] > 1:
-        t = t.contiguous()
     return t if t.dim() == 2 else t.reshape(-1, shape[-1])
