@@ -31,14 +31,19 @@ __device__ __forceinline__ Pack<T, V> conv_input(const ConvSeqArgs& a, int b, in
     else p.zero();
     return p;
 }
-// a channel vector's taps and bias
+// the taps and bias of the n channels (at most V) from ch on
 template <int V, int K>
-__device__ __forceinline__ void conv_weights(const float* w, const float* bias, int ch, int D, float (&wk)[K][V], float (&b)[V]) {
+__device__ __forceinline__ void conv_weights(const float* w, const float* bias, int ch, int n, float (&wk)[K][V], float (&b)[V]) {
+    Pack<float, V * K> rows;
+    rows.load_n(w + (size_t)ch * K, n >= V ? V * K : n * K);
+    Pack<float, V> bs;
+    bs.zero();
+    if (bias) bs.load_n(bias + ch, n);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        b[v] = bias && ch + v < D ? bias[ch + v] : 0.f;
+        b[v] = bs.get(v);
 #pragma unroll
-        for (int k = 0; k < K; ++k) wk[k][v] = ch + v < D ? w[(ch + v) * K + k] : 0.f;
+        for (int k = 0; k < K; ++k) wk[k][v] = rows.get(v * K + k);
     }
 }
 
@@ -61,7 +66,7 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restr
     if (t0 >= t1) return;
     const int n = TAIL ? a.D - ch : V;
     float w[K][V], bias[V];
-    conv_weights<V, K>(a.w, a.bias, ch, a.D, w, bias);
+    conv_weights<V, K>(a.w, a.bias, ch, n, w, bias);
     T* out = y + ((size_t)b * a.L + t0) * a.D + ch;
     const int tend = min(t1, len);
     float win[K - 1][V];
@@ -141,7 +146,7 @@ __global__ __launch_bounds__(256) void conv_seq_bwd_kernel(ConvSeqArgs a, const 
     const int len = seq_len(a.lengths, b, a.L);
     const int n = TAIL ? a.D - ch : V;
     float w[K][V], bias[V], dw[K][V], db[V];
-    conv_weights<V, K>(a.w, a.bias, ch, a.D, w, bias);
+    conv_weights<V, K>(a.w, a.bias, ch, n, w, bias);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         db[v] = 0.f;
@@ -295,7 +300,7 @@ __global__ __launch_bounds__(256) void conv_seq_step_kernel(const T* __restrict_
     for (int i = 0; i < K - 1; ++i) r[i].load_n(st + (size_t)i * D, n);
     r[K - 1].load_n(x + row * xb + ch, n);
     float wk[K][V], b[V];
-    conv_weights<V, K>(w, bias, ch, D, wk, b);
+    conv_weights<V, K>(w, bias, ch, n, wk, b);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         float s = b[v];
@@ -356,9 +361,10 @@ struct ConvSeqPlan {
 };
 
 // threads along the channels: as many (a power of two, at most a wave) as there are channel vectors; the rest of the
-// block along time.  steps = rows per thread; the launch should give every CU a few blocks, so short or narrow inputs
-// take fewer rows per thread.
-ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d, int most_steps) {
+// block along time.  steps = rows per thread: 32 as long as that leaves two blocks a CU, down to 8 on short or narrow
+// inputs, where each row that two threads share is read twice (backward of 32 x 501 x 768 fp32: 36 us with 16 rows and 768
+// blocks, 41 with 8; forward of 8 x 4096 x 2048 bf16: 43.5 us with 32 rows, 45.6 with 16).
+ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d) {
     ConvSeqPlan p;
     p.V = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
     const int nv = (d.channels + p.V - 1) / p.V;
@@ -366,8 +372,8 @@ ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d, int most_steps) {
     while ((1 << p.cw_log2) < nv && p.cw_log2 < 6) ++p.cw_log2;
     p.nblk_c = (nv + (1 << p.cw_log2) - 1) >> p.cw_log2;
     const int nseg = 256 >> p.cw_log2;
-    p.steps = most_steps;
-    while (p.steps > 8 && (long long)d.batch * p.nblk_c * ((d.length + p.steps * nseg - 1) / (p.steps * nseg)) < 1024) p.steps /= 2;
+    p.steps = 32;
+    while (p.steps > 8 && (long long)d.batch * p.nblk_c * ((d.length + p.steps * nseg - 1) / (p.steps * nseg)) < 512) p.steps /= 2;
     p.nblk_t = (d.length + p.steps * nseg - 1) / (p.steps * nseg);
     return p;
 }
@@ -453,7 +459,7 @@ struct RunStep {
     }
 };
 
-constexpr int kFwdSteps = 16, kBwdSteps = 32;
+
 
 }  // namespace
 }  // namespace unetmi
@@ -469,7 +475,7 @@ int unetmi_seq_conv_fwd(const UnetmiSeqConvDesc* d, const void* x, const float* 
     if (d->batch == 0) return UNETMI_OK;
     if (!weight || (d->length > 0 && (!x || !y))) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_fwd: null tensor pointer");
     if (d->length == 0 && !state_out) return UNETMI_OK;
-    const ConvSeqPlan p = conv_plan(*d, kFwdSteps);
+    const ConvSeqPlan p = conv_plan(*d);
     if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_fwd: too many steps");
     return conv_dispatch<RunFwd>(*d, conv_args(*d, p, x, weight, bias, state, lengths), p, y, state_out,
                                  static_cast<hipStream_t>(stream));
@@ -477,7 +483,7 @@ int unetmi_seq_conv_fwd(const UnetmiSeqConvDesc* d, const void* x, const float* 
 
 size_t unetmi_seq_conv_bwd_workspace_bytes(const UnetmiSeqConvDesc* d) {
     if (conv_check(d, "seq_conv_bwd") != UNETMI_OK) return 0;
-    const ConvSeqPlan p = conv_plan(*d, kBwdSteps);
+    const ConvSeqPlan p = conv_plan(*d);
     return (size_t)(d->batch > 0 ? d->batch : 1) * (p.nblk_t > 0 ? p.nblk_t : 1) * d->channels * (d->taps + 1) * sizeof(float);
 }
 
@@ -490,7 +496,7 @@ int unetmi_seq_conv_bwd(const UnetmiSeqConvDesc* d, const void* x, const float* 
     if (!weight || !dweight || !dbias || !ws || (d->length > 0 && (!x || !dy || !dx)))
         return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: null tensor pointer");
     if (ws_bytes < unetmi_seq_conv_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "seq_conv_bwd: workspace too small");
-    const ConvSeqPlan p = conv_plan(*d, kBwdSteps);
+    const ConvSeqPlan p = conv_plan(*d);
     if (p.nblk_t > 65535) return api_fail(UNETMI_E_UNSUPPORTED, "seq_conv_bwd: too many steps");
     return conv_dispatch<RunBwd>(*d, conv_args(*d, p, x, weight, bias, state, lengths), p, *d, dy, dstate_out, dx, dstate,
                                  dweight, dbias, static_cast<float*>(ws), static_cast<hipStream_t>(stream));

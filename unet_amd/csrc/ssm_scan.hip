@@ -109,6 +109,20 @@ __device__ __forceinline__ void window_store(T v, __amdgpu_buffer_rsrc_t rs, int
     else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, v), rs, voff, soff, 0);
 }
 
+template <int S>
+__device__ __forceinline__ void window_store_states(const float (&h)[S], __amdgpu_buffer_rsrc_t rs, int voff) {
+    typedef int i32x2 __attribute__((ext_vector_type(2)));
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    if constexpr (S == 1) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, h[0]), rs, voff, 0, 0);
+    else if constexpr (S == 2) __builtin_amdgcn_raw_buffer_store_b64(i32x2{__builtin_bit_cast(int, h[0]), __builtin_bit_cast(int, h[1])}, rs, voff, 0, 0);
+    else {
+#pragma unroll
+        for (int s = 0; s < S; s += 4)
+            __builtin_amdgcn_raw_buffer_store_b128(i32x4{__builtin_bit_cast(int, h[s]), __builtin_bit_cast(int, h[s + 1]),
+                                                         __builtin_bit_cast(int, h[s + 2]), __builtin_bit_cast(int, h[s + 3])}, rs, voff, 4 * s, 0);
+    }
+}
+
 // A lane's steps of a tile: 4i + q of its channel, i = 0..STEPS/4-1.
 template <class T, int STEPS>
 struct Column {
@@ -177,13 +191,16 @@ struct Shared {
 template <class T>
 __device__ __forceinline__ float at(const void* p, long long i) { return widen(static_cast<const T*>(p)[i]); }
 
-// Forward.  STATE_ONLY: the first pass over a time axis that is split into chunks: the chunk's last state from zero and
-// the sum of its steps (the product of its decays is exp(A sum dt)).  Else the whole operator on a chunk, starting from
-// the states of the chunks before it.  A tile's inputs are loaded while the tile before it is computed, B and C into the
+// Forward.  kStates: the first pass over a time axis that is split into chunks: the chunk's last state from zero and the
+// sum of its steps (the product of its decays is exp(A sum dt)).  Else the whole operator on a chunk, starting from the
+// states of the chunks before it; kMarks also saves the states that the backward kernel starts its tiles from.  A tile's inputs are loaded while the tile before it is computed, B and C into the
 // other half of LDS: one barrier a tile.
-template <class T, int S, bool STATE_ONLY>
+enum ScanPass { kStates, kOutputs, kMarks };
+
+template <class T, int S, ScanPass PASS>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
     constexpr int NP = 4 * S, MK = mark_steps<S>();
+    constexpr bool STATE_ONLY = PASS == kStates;
     __shared__ float lds_b[2][kTile * NP], lds_c[STATE_ONLY ? 1 : 2][STATE_ONLY ? 1 : kTile * NP];
     const Place p = place(a, blockIdx.z);
     const int chunk = blockIdx.y, t0 = chunk * a.chunk, t1 = min(t0 + a.chunk, a.L), tend = min(t1, p.len);
@@ -236,8 +253,9 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < kTile / 4; ++i) {
-            if (!STATE_ONLY && a.marks && (4 * i) % MK == 0 && dt0 + 4 * i < left && p.live)
-                store_padded<S>(h, a.marks + (((size_t)p.b * a.nmark + (t0 + dt0 + 4 * i) / MK) * a.D + p.ch) * NP, p.q);
+            if (PASS == kMarks && (4 * i) % MK == 0)
+                window_store_states<S>(h, window(a.marks + ((size_t)p.b * a.nmark + (t0 + dt0 + 4 * i) / MK) * a.D * NP),
+                                       p.live && dt0 + 4 * i < left ? (p.ch * NP + p.q * S) * 4 : kOutside);
             dt[i] = dt0 + 4 * i + p.q < left ? dt[i] : 0.f;
             const float u = dt[i] * x[i];
             sdt += dt[i];
@@ -578,17 +596,17 @@ __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs 
 template <class T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC,
                                                       const int* __restrict__ lengths, long long rows, int L, int G, int tpg, int N, int NP) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;             // (row, which, n)
-    const int per = 2 * NP;
-    const long long row = i / per;
-    if (row >= rows) return;
-    const int r = (int)(i - row * per), n = r % NP;
-    if (n >= N) return;
-    const long long bt = row / G;
-    float s = 0.f;
-    if (!lengths || bt % L < lengths[bt / L])
-        for (int k = 0; k < tpg; ++k) s += part[(row * tpg + k) * per + r];
-    (r < NP ? dB : dC)[row * N + n] = (T)s;
+    const int per = 2 * NP;                                           // a power of two: (which, n)
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (long long)gridDim.x * 256) {
+        const long long row = i / per;
+        const int r = (int)(i - row * per), n = r & (NP - 1);
+        if (n >= N) continue;
+        const long long bt = row / G;
+        float s = 0.f;
+        if (!lengths || bt % L < lengths[bt / L])
+            for (int k = 0; k < tpg; ++k) s += part[(row * tpg + k) * per + r];
+        (r < NP ? dB : dC)[row * N + n] = (T)s;
+    }
 }
 
 // One token of every row; state [slots, D, N] is read and written once: 8N bytes a channel against 7N operations, HBM
@@ -734,11 +752,13 @@ struct RunScan {
         const dim3 block(256);
         if (p.nchunk > 1) {
             // the last chunk's summary is never read
-            hipLaunchKernelGGL((scan_fwd_kernel<T, S, true>), dim3(d.groups * p.tpg, p.nchunk - 1, d.batch), block, 0, s, a);
+            hipLaunchKernelGGL((scan_fwd_kernel<T, S, kStates>), dim3(d.groups * p.tpg, p.nchunk - 1, d.batch), block, 0, s, a);
             const int rc = launched("ssm_scan_fwd states");
             if (rc != UNETMI_OK) return rc;
         }
-        hipLaunchKernelGGL((scan_fwd_kernel<T, S, false>), dim3(d.groups * p.tpg, p.nchunk, d.batch), block, 0, s, a);
+        const dim3 grid(d.groups * p.tpg, p.nchunk, d.batch);
+        if (a.marks) hipLaunchKernelGGL((scan_fwd_kernel<T, S, kMarks>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((scan_fwd_kernel<T, S, kOutputs>), grid, block, 0, s, a);
         return launched("ssm_scan_fwd");
     }
 };
@@ -755,7 +775,8 @@ struct RunScanBwd {
         if ((rc = launched("ssm_scan_bwd")) != UNETMI_OK) return rc;
         const long long rows = (long long)d.batch * d.length * d.groups, threads = rows * 2 * p.NP;
         if (threads) {
-            hipLaunchKernelGGL((scan_bc_kernel<T>), dim3((unsigned)((threads + 255) / 256)), block, 0, s, a.pBC, static_cast<T*>(dB),
+            const long long blocks = (threads + 255) / 256;
+            hipLaunchKernelGGL((scan_bc_kernel<T>), dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), block, 0, s, a.pBC, static_cast<T*>(dB),
                                static_cast<T*>(dC), a.lengths, rows, d.length, d.groups, p.tpg, d.state, p.NP);
             if ((rc = launched("ssm_scan_bwd B C")) != UNETMI_OK) return rc;
         }
