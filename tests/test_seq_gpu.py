@@ -430,6 +430,53 @@ def test_saved_state_and_a_second_backward(device):
         y.sum().backward()
 
 
+def test_gradients_under_create_graph(device):
+    """create_graph gives the same gradients; asking for a second derivative says that there is none."""
+    from unet_amd import norm, ssm
+    x = rnd((1, 20, 64), 1).to(device).requires_grad_()
+    w = rnd((64, 4), 2).to(device).requires_grad_()
+    bc = rnd((1, 20, 4), 3).to(device)
+    for name, call in (("causal_conv", lambda: ssm.causal_conv(x, w)),
+                       ("selective_scan", lambda: ssm.selective_scan(x, x, -torch.ones(64, 4, device=device), bc, bc)),
+                       ("block_norm", lambda: norm.block_norm(x, gate=x))):
+        plain, = torch.autograd.grad(call().sum(), x)
+        g, = torch.autograd.grad(call().sum(), x, create_graph=True)
+        assert torch.equal(plain, g.detach()) and g.requires_grad
+        with pytest.raises(RuntimeError, match=name + " can be differentiated once only"):
+            g.sum().backward()
+
+
+def test_leaves_that_want_no_gradient(device):
+    """Only some inputs want gradients, optional ones among them given and not: each gets its own."""
+    from unet_amd import norm, ssm
+    p, _, dy, _ = scan_inputs(1, 30, 64, 16, 1, True, True, True, True, None, F32, True)
+    q = {k: t.to(device) for k, t in p.items()}
+    every = {k: t.clone().requires_grad_() for k, t in q.items()}
+    want = dict(zip(every, torch.autograd.grad(ssm.selective_scan(**every), list(every.values()), dy.to(device))))
+    for some in (["state"], ["z", "A"], ["C"], ["dt_bias", "state"]):
+        args = {k: (t.clone().requires_grad_() if k in some else t) for k, t in q.items()}
+        got = torch.autograd.grad(ssm.selective_scan(**args), [args[k] for k in some], dy.to(device))
+        assert all(torch.equal(g, want[k]) for k, g in zip(some, got))
+    # without D the places of what follows it move up
+    args = {k: (t.clone().requires_grad_() if k == "dt_bias" else t) for k, t in q.items() if k not in ("D", "z")}
+    g, = torch.autograd.grad(ssm.selective_scan(**args), args["dt_bias"], dy.to(device))
+    ref = scan64(**{k: t for k, t in p.items() if k not in ("D", "z")}, dy=dy)
+    assert torch.allclose(g.cpu().double(), ref["d_dt_bias"], rtol=1e-3, atol=1e-4)
+    s = rnd((1, 3, 64), 5).to(device).requires_grad_()
+    w = rnd((64, 4), 2).to(device)
+    a, = torch.autograd.grad(ssm.causal_conv(q["x"], w, state=s), s, dy.to(device))
+    b = torch.autograd.grad(ssm.causal_conv(q["x"].requires_grad_(), w, torch.zeros(64, device=device).requires_grad_(), state=s), s, dy.to(device))[0]
+    assert torch.equal(a, b)
+    r = rnd((5, 64), 6).to(device).requires_grad_()
+    pre = rnd((64,), 7).to(device).requires_grad_()
+    x = rnd((5, 64), 8).to(device)
+    gr, gp = torch.autograd.grad(norm.block_norm(x, residual=r, pre_weight=pre)[1].sum(), (r, pre))
+    full = norm64(x, None, None, r, None, pre, 1e-6, None, torch.ones(5, 64))
+    room = norm64(x, None, None, r, None, pre, 1e-6, None, torch.ones(5, 64), magnitude=True)
+    held(gr, full["d_residual"], room["d_residual"], 192, "d residual")
+    held(gp, full["d_pre"], room["d_pre"], 200, "d pre_weight")
+
+
 def test_refusals_on_the_device(device):
     from unet_amd import norm, ssm
     from unet_amd._lib import UnetmiError

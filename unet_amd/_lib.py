@@ -7,7 +7,7 @@ the header declares.  There is no CPU or eager fallback.
 
 import ctypes
 import os
-import struct
+
 import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -119,12 +119,6 @@ class NormDesc(ctypes.Structure):
     """struct UnetmiNormDesc."""
     _fields_ = [("rows", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("channels", "dtype", "residual_dtype")] + [
         ("eps", ctypes.c_float)] + [(n, ctypes.c_int64) for n in ("x_stride", "gate_stride", "residual_stride")]
-
-
-# The same layouts for struct.pack: a descriptor per call costs a tenth of building a ctypes structure.
-PACK_SEQ_CONV, PACK_SCAN, PACK_NORM = struct.Struct("@6i4q"), struct.Struct("@8i14q"), struct.Struct("@q3if3q")
-for _packer, _structure in ((PACK_SEQ_CONV, SeqConvDesc), (PACK_SCAN, ScanDesc), (PACK_NORM, NormDesc)):
-    assert _packer.size == ctypes.sizeof(_structure)
 
 
 E_BAD_DESC, E_BAD_ARG, E_HIP, E_UNSUPPORTED = -1, -2, -3, -4
@@ -240,7 +234,7 @@ def _load():
     lib.unetmi_comm_world.argtypes = []
     lib.unetmi_allreduce_f32.argtypes = [fp, sz, vp]
     lib.unetmi_comm_destroy.argtypes = []
-    conv = scan = norm = vp                       # a byref() of the structure, or its packed bytes
+    conv, scan, norm = ctypes.POINTER(SeqConvDesc), ctypes.POINTER(ScanDesc), ctypes.POINTER(NormDesc)
     lib.unetmi_seq_conv_fwd.argtypes = [conv] + [vp] * 8
     lib.unetmi_seq_conv_bwd.argtypes = [conv] + [vp] * 12 + [sz, vp]
     lib.unetmi_seq_conv_step.argtypes = [conv] + [vp] * 4 + [ci] + [vp] * 3
