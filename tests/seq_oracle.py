@@ -78,7 +78,9 @@ def scan64(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=No
     size = mag(step)
     ends = ends_of(lengths, batch, L)
     h = torch.zeros(batch, ch, N, dtype=torch.float64) if state is None else mag(state)
-    gate = torch.ones_like(x) if z is None else (mag(z) * sig(z) * (1 + mag(z) if magnitude else 1))
+    # fp32 has no normal number below 2^-126: a gate's sigmoid that small may come out as zero, off by up to 2^-126, which is
+    # 2^-102 in units of 2^-24 (z below -87; the product of z, the sigmoid and y can still be a normal number)
+    gate = torch.ones_like(x) if z is None else (mag(z) * (sig(z) + 2.0 ** -102) * (1 + mag(z)) if magnitude else z * sig(z))
     out = {"y": torch.zeros_like(x)}
     hs, bare = [h], torch.zeros_like(x)
     decay = lambda t: torch.exp(step[:, t, :, None] * A)  # noqa: E731

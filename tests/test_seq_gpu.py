@@ -110,6 +110,22 @@ def test_causal_conv_step_continues_a_prompt(device, rows, slots_n, D, K, dtype)
         assert not torch.equal(cache[slots[1]], before[slots[1]])
 
 
+def test_causal_conv_ignores_what_lies_behind_the_end(device):
+    """NaN and infinities behind the sequences' ends, in the inputs and in the output's gradient, reach nothing."""
+    from unet_amd import ssm
+    x, w, b, s, n, dy, ds = conv_inputs(4, 50, 72, 4, True, True, [50, 0, 2, 33], F32)
+    want, room = conv64(x, w, b, s, n, True, dy, ds), conv64(x, w, b, s, n, True, dy, ds, magnitude=True)
+    for i, k in enumerate(n.tolist()):
+        x[i, k:], dy[i, k:] = float("nan"), float("inf")
+    leaves = [t.to(device).requires_grad_() for t in (x, w, b, s)]
+    for lengths in (n, n.long() + torch.tensor([2 ** 40, -(2 ** 40), 0, 0]), n.to(torch.int16)):
+        y, out = ssm.causal_conv(leaves[0], leaves[1], leaves[2], state=leaves[3], lengths=lengths.to(device), return_state=True)
+        grads = torch.autograd.grad((y, out), leaves, (dy.to(device), ds.to(device)))
+        held(y, want["y"], room["y"], 16, "y")
+        for g, k, count in zip(grads, ("dx", "dw", "db", "dstate"), (24, 224, 224, 24)):
+            held(g, want[k], room[k], count, k)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # selective scan
 # ---------------------------------------------------------------------------------------------------------------------
@@ -257,6 +273,55 @@ def test_selective_scan_prompt_in_pieces(device):
     held(state, end.cpu().double(), room["state"], 2 * (2 * 300 + 80), "state")
 
 
+def test_selective_scan_at_the_ends_of_the_ranges(device):
+    """Step sizes from e^-60 to 80 and gates far out on both sides: nothing overflows on the way to a finite value.  The
+    softplus of v carries the rounding of v's own exponent, |v| 2^-24 of it, hence the count."""
+    from unet_amd import ssm
+    p, _, dy, _ = scan_inputs(1, 64, 64, 16, 1, True, True, False, False, None, F32, True)
+    p["dt"] = torch.linspace(-60, 80, 64 * 64).view(1, 64, 64)
+    p["z"] = torch.linspace(120, -120, 64 * 64).view(1, 64, 64)
+    want, room = scan64(**p, dy=dy), scan64(**p, dy=dy, magnitude=True)
+    leaves = {k: t.to(device).requires_grad_() for k, t in p.items() if t is not None}
+    y = ssm.selective_scan(**leaves)
+    held(y, want["y"], room["y"], 2 * 64 + 16 + 64 + 200, "y")
+    for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy.to(device))):
+        held(g, want["d_" + k], room["d_" + k], 4 * 64 + 2 * 16 + 96 + 400 + 64, "d " + k)
+
+
+def test_more_than_two_to_the_31_elements(device):
+    """Sequences, caches and rows whose last elements lie beyond 2^31: the same bits as the last part on its own."""
+    from unet_amd import norm, ssm
+    ch, L, tail = 131072, 16416, 32
+    gen = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn((1, L, ch), generator=gen, device=device, dtype=BF16)
+    w = torch.randn((ch, 4), generator=gen, device=device)
+    y, end = ssm.causal_conv(x, w, return_state=True)
+    _, before = ssm.causal_conv(x[:, :L - tail], w, return_state=True)
+    y1, end1 = ssm.causal_conv(x[:, L - tail:], w, state=before, return_state=True)
+    assert torch.equal(y[:, L - tail:], y1) and torch.equal(end, end1)
+    del y, y1
+    A = -torch.rand((ch, 4), generator=gen, device=device) - 0.5
+    B, C = (torch.randn((1, L, 4), generator=gen, device=device, dtype=BF16) for _ in range(2))
+    y, end = ssm.selective_scan(x, x, A, B, C, return_state=True)
+    _, before = ssm.selective_scan(x[:, :L - tail], x[:, :L - tail], A, B[:, :L - tail], C[:, :L - tail], return_state=True)
+    y1, end1 = ssm.selective_scan(x[:, L - tail:], x[:, L - tail:], A, B[:, L - tail:], C[:, L - tail:], state=before, return_state=True)
+    assert torch.equal(y[:, L - tail:], y1) and torch.equal(end, end1)
+    del y, y1
+    rows = x.view(-1, 8192)
+    pre = torch.rand((8192,), generator=gen, device=device)
+    r, n = norm.block_norm(rows, residual=rows, pre_weight=pre)
+    r1, n1 = norm.block_norm(rows[-7:], residual=rows[-7:], pre_weight=pre)
+    assert torch.equal(r[-7:], r1) and torch.equal(n[-7:], n1)
+    del r, n, rows
+    cache = torch.zeros((4100, ch, 4), device=device)                  # 2.1e9 states
+    slots = torch.tensor([4099, 0], device=device)
+    token = x[0, :2]
+    y = ssm.selective_scan_step(token, token, A, B[0, :2], C[0, :2], cache, slots=slots)
+    small = torch.zeros((2, ch, 4), device=device)
+    assert torch.equal(y, ssm.selective_scan_step(token, token, A, B[0, :2], C[0, :2], small))
+    assert torch.equal(cache[4099], small[0]) and torch.equal(cache[0], small[1]) and not cache[1:4099].any()
+
+
 def test_selective_scan_long_and_wide_offsets(device):
     """Element offsets beyond 2^31: a batch of expanded (stride 0) rows and a slice far into a large buffer."""
     from unet_amd import ssm
@@ -394,6 +459,50 @@ def test_block_gradients_in_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(kept, eager)), [i for i, (a, b) in enumerate(zip(kept, eager)) if not torch.equal(a, b)]
 
 
+def test_tokens_in_a_graph(device):
+    """A block's token step captured once and replayed over a growing stream, two graphs in turn on two caches, with eager
+    work between: every token is the eager one, bit for bit."""
+    from unet_amd import norm, ssm
+    p = {k: v.detach() for k, v in block_params(64, device).items()}
+    c, n = p["in"].shape[1] // 2, p["A"].shape[1]
+
+    def token(x, conv, state, slots):
+        xz = norm.block_norm(x, post_weight=p["norm"]) @ p["in"]
+        u = ssm.causal_conv_step(xz[:, :c], conv, p["conv_w"], p["conv_b"], slots=slots)
+        dbc = u @ p["dbc"]
+        y = ssm.selective_scan_step(u, dbc[:, :1] * p["dt_w"], p["A"], dbc[:, 1:1 + n], dbc[:, 1 + n:], state, D=p["D"], z=xz[:, c:],
+                                    dt_bias=p["dt_b"], slots=slots)
+        return norm.block_norm(y @ p["out"], residual=x, scale=p["scale"], pre_weight=p["norm"])
+
+    def cache(seed):
+        return rnd((9, 3, c), seed).to(device), rnd((9, c, n), seed + 1).to(device)
+
+    slots = torch.tensor([4, 0, -1, 8, 2], dtype=torch.int32, device=device)
+    xs = [rnd((5, 64), 60 + i).to(device) for i in range(8)]
+    caches, eager = [cache(50), cache(52)], [cache(50), cache(52)]
+    x = xs[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        token(x, *cache(54), slots)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(token(x, *caches[k], slots))
+        graphs.append(g)
+    for i, new in enumerate(xs):
+        k = i % 2
+        want = token(new, *eager[k], slots)
+        x.copy_(new)
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs[k], want)), i
+        assert all(torch.equal(a, b) for a, b in zip(caches[k], eager[k])), i
+
+
 def test_two_streams_at_once(device):
     """Calls on two streams share nothing."""
     from unet_amd import ssm
@@ -505,6 +614,12 @@ def test_refusals_on_the_device(device):
     with pytest.raises(UnetmiError, match="fewer slots"):
         ssm.selective_scan_step(torch.zeros(3, 8, device=device), torch.zeros(3, 8, device=device), A, torch.zeros(3, 2, device=device),
                                 torch.zeros(3, 2, device=device), torch.zeros(2, 8, 2, device=device))
+    with pytest.raises(ValueError, match="act is True or False"):
+        ssm.causal_conv(x, torch.zeros(8, 4, device=device), act="none")
+    with pytest.raises(ValueError, match="contiguous"):
+        ssm.causal_conv_step(x[0], torch.zeros(4, 8, 3, device=device).transpose(1, 2), torch.zeros(8, 4, device=device))
+    with pytest.raises(ValueError, match="state must"):
+        ssm.selective_scan_step(x[0], x[0], A, bc[0], bc[0], torch.zeros(4, 8, 2, device=device, dtype=BF16))
     with pytest.raises(ValueError, match="residual"):
         norm.block_norm(x, pre_weight=torch.ones(8, device=device))
     with pytest.raises(UnetmiError, match="8192"):

@@ -555,4 +555,7 @@ TORCH_LIBRARY_IMPL(unetmi, Autograd, m) {
     m.impl("seq_conv", seq_conv_autograd);
     m.impl("ssm_scan", ssm_scan_autograd);
     m.impl("block_norm", block_norm_autograd);
+    // the tokens' and the backward ops record nothing
+    for (const char* name : {"seq_conv_step", "ssm_scan_step", "seq_conv_bwd", "ssm_scan_bwd", "block_norm_bwd"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
 }
