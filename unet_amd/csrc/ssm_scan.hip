@@ -193,8 +193,10 @@ __device__ __forceinline__ float at(const void* p, long long i) { return widen(s
 
 // Forward.  kStates: the first pass over a time axis that is split into chunks: the chunk's last state from zero and the
 // sum of its steps (the product of its decays is exp(A sum dt)).  Else the whole operator on a chunk, starting from the
-// states of the chunks before it; kMarks also saves the states that the backward kernel starts its tiles from.  A tile's inputs are loaded while the tile before it is computed, B and C into the
-// other half of LDS: one barrier a tile.
+// states of the chunks before it; kMarks also saves the states that the backward kernel starts its tiles from.  A tile's
+// inputs are loaded while the tile before it is computed, B and C go into the other half of LDS: one barrier a tile.
+// Measured: 1 x 8192 x 2048 channels x 16 states bf16 58 + 88 us in 32 chunks, the vector units 88 and 81 % busy with 22 and
+// 33 instructions a step and wave; 128 x 501 x 256 fp32 with marks 110 us (3.6 TB/s); 4 x 4096 x 2048 bf16 110 + 181 us.
 enum ScanPass { kStates, kOutputs, kMarks };
 
 template <class T, int S, ScanPass PASS>
@@ -301,7 +303,8 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 }
 
 // The first backward pass over a split time axis: the adjoint that a chunk hands to the chunk before it, from zero,
-// and the sum of its steps.  Built like the forward pass, from the chunk's last tile to its first.
+// and the sum of its steps.  Built like the forward pass, from the chunk's last tile to its first.  4 x 4096 x 2048 bf16 in
+// eight chunks: 125 us, vector units 90 % busy.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_bwd_state_kernel(ScanArgs a) {
     constexpr int NP = 4 * S;
@@ -416,7 +419,10 @@ __device__ __forceinline__ void channel_sums(float (&v)[MK][S]) {
 //     d raw = (A . w + du x) sigmoid(raw),  dx = du dt + D dy',  dA = sum w dt
 // A channel's shares of dB and dC take the registers of its a_t and h_t; they are summed over the wave by lane exchanges
 // and over the block's waves through LDS, and the block writes one row of partial sums per step.  One barrier a tile: the
-// LDS areas are used in turn, and a tile's sums are taken after the next one's barrier.
+// LDS areas are used in turn, and a tile's sums are taken after the next one's barrier.  Tiles of eight steps (16 states)
+// keep the kernel at 191 registers and two waves a SIMD; sixteen steps spilled there (817 us for 128 x 501 x 256 fp32) and
+// took 357 us at one wave.  Measured: 255 us there, 470 us for 4 x 4096 x 2048 bf16, vector units 82 and 86 % busy with 98
+// instructions a step and wave (16 of them the exchanges; the same sums as fp32 matrix products took 373 and 694 us).
 template <class T, int S>
 __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs a) {
     constexpr int NP = 4 * S, MK = mark_steps<S>(), NI = MK / 4, RED = MK * 2 * NP;
@@ -592,7 +598,7 @@ __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs 
     }
 }
 
-// dB, dC [B, L, G, N] from the blocks' partial sums [B, L, G, tpg, 2, NP]
+// dB, dC [B, L, G, N] from the blocks' partial sums [B, L, G, tpg, 2, NP]: 4 x 4096 steps of 32 blocks, 67 MB in 20 us
 template <class T>
 __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ part, T* __restrict__ dB, T* __restrict__ dC,
                                                       const int* __restrict__ lengths, long long rows, int L, int G, int tpg, int N, int NP) {
@@ -610,7 +616,8 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
 }
 
 // One token of every row; state [slots, D, N] is read and written once: 8N bytes a channel against 7N operations, HBM
-// bound.  A block takes a row's blocks of 64 channels in turn (of one group: B and C are loaded once), so that the check of
+// bound: 256 rows x 2048 channels x 16 states in 18.4 us (3.9 TB/s; 39 with a block per 64 channels and single loads); one
+// row of 1280 channels in 4.  A block takes a row's blocks of 64 channels in turn (of one group: B and C are loaded once), so that the check of
 // the row's slot against the rows before it is paid once for several of them.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, int parts, const int* __restrict__ slots, int nslots, float* __restrict__ state) {

@@ -9,6 +9,10 @@ layernorm_w_act); a block whose channels are innermost -- a state space layer, u
 from . import seq_ops as _ops
 
 
+def _packed(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
 def block_norm(x, gate=None, post_weight=None, residual=None, scale=None, pre_weight=None, eps=1e-6):
     """x [..., channels] (channels <= 8192) -> p; with a residual -> r; with a residual and pre_weight -> (r, n).
 
@@ -18,15 +22,15 @@ def block_norm(x, gate=None, post_weight=None, residual=None, scale=None, pre_we
     if residual is None and (scale is not None or pre_weight is not None):
         raise ValueError("unet_amd.norm: scale and pre_weight belong to a residual stream")
     shape = x.shape
-    for t in (gate, residual):
-        if t is not None and t.shape != shape:
-            raise ValueError("unet_amd.norm: x, gate and residual have one shape, got {} and {}".format(tuple(shape), tuple(t.shape)))
+    rows = len(shape) == 2
+    if not rows:                                          # [..., channels] as rows: a copy only where they are not evenly spaced
+        for t in (gate, residual):
+            if t is not None and t.shape != shape:
+                raise ValueError("unet_amd.norm: x, gate and residual have one shape, got {} and {}".format(tuple(shape), tuple(t.shape)))
+        x, gate, residual = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, gate, residual))
     if scale is not None and scale.numel() == 1:
         scale = scale.reshape(1).expand(shape[-1])
-    if len(shape) != 2:                                   # [..., channels] as rows: a copy only where they are not evenly spaced
-        x, gate, residual = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, gate, residual))
-    weights = [t if t is None or t.is_contiguous() else t.contiguous() for t in (post_weight, scale, pre_weight)]
-    out, out_n = _ops.block_norm(x, gate, weights[0], residual, weights[1], weights[2], eps)
-    if len(shape) != 2:
+    out, out_n = _ops.block_norm(x, gate, _packed(post_weight), residual, _packed(scale), _packed(pre_weight), eps)
+    if not rows:
         out, out_n = out.view(shape), out_n if pre_weight is None else out_n.view(shape)
     return out if pre_weight is None else (out, out_n)
