@@ -7,7 +7,7 @@
 // HBM bounds both directions.  A thread holds E elements of a row in fp32: eight, rows of up to 512 elements one wave and
 // wider ones a block of up to eight waves; sixteen beyond 4096 elements.  Blocks walk over rows: the weights stay in registers, and in the
 // backward kernel so do their gradients' partial sums, added up in a fixed order by a second kernel.  Measured: forward
-// 16387 x 2048 bf16 67 us (5.0 TB/s), 16032 x 1285 fp32 77 us (5.3 TB/s), its backward 150 us (4.4 TB/s) and 6 for the sums;
+// 16387 x 2048 bf16 61 us (5.5 TB/s), 16032 x 1285 fp32 81 us (5.1 TB/s), its backward 132 us (5.0 TB/s) and 6 for the sums;
 // 64 rows of 2048 in 4 us.
 #include "seq_common.hpp"
 
@@ -235,6 +235,8 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
 
 namespace {
 
+// Elements a thread: sixteen where eight would need more than eight waves a row -- blocks of sixteen waves leave the backward
+// kernel 128 registers, which spilled (16032 x 1285 fp32 bounded for them: 286 us against 150).
 int norm_elems(const UnetmiNormDesc& d) { return d.channels <= 4096 ? 8 : 16; }
 
 struct NormPlan {
@@ -252,9 +254,11 @@ NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
     return p;
 }
 
-// resident work: about 32 waves per CU forward; half of that backward, whose partial sums cost 12 bytes a column and worker
-long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 32 / (p.width * p.per_block / 64); }
-long long bwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 8 / (p.width * p.per_block / 64); }
+// Waves per CU: forward 64, about three times what is resident, so that CUs that end early find work (16387 x 2048 bf16: 61 us,
+// 67 with 32 and 65 with 16; 16032 x 1285 fp32: 81, 78 and 85).  Backward 12, what is resident, since every block more costs
+// 12 bytes a column of partial sums (16032 x 1285 fp32: 132 us and 6 for the sums; 8 waves 153, 16 waves 173, 24 141 and 12).
+long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 64 / (p.width * p.per_block / 64); }
+long long bwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 12 / (p.width * p.per_block / 64); }
 
 int norm_check(const UnetmiNormDesc* d, const char* what) {
     const std::string w = what;

@@ -49,7 +49,8 @@ __device__ __forceinline__ void conv_weights(const float* w, const float* bias, 
     }
 }
 
-// TAIL: the channels are no multiple of V, the last vector of a row holds fewer.
+// TAIL: the channels are no multiple of V, the last vector of a row holds fewer (guarded accesses for every width took 51 us
+// where the whole vectors take 43).
 template <class T, int V, int K, bool ACT, bool TAIL>
 __global__ __launch_bounds__(256) void conv_seq_kernel(ConvSeqArgs a, T* __restrict__ y, T* __restrict__ state_out) {
     const int cw = 1 << a.cw_log2;
