@@ -580,7 +580,7 @@ int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float*
  * (NULL: zeros); state_out may be NULL and must not be `state`.  The inputs' steps are at most UNETMI_SEQ_MAX_STEP elements
  * apart.  marks (NULL for inference): the states that the backward
  * call starts its tiles from, unetmi_ssm_scan_marks_bytes of them.  States, decays and sums are fp32 throughout. */
-#define UNETMI_SEQ_MAX_STEP (1 << 25)
+#define UNETMI_SEQ_MAX_STEP (1 << 24)
 typedef struct UnetmiScanDesc {
     int32_t batch, length, channels, state, groups, dtype, softplus, reserved;
     int64_t x_stride[2], dt_stride[2], z_stride[2], dy_stride[2];    /* between sequences, between steps */

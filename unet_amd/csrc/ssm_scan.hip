@@ -15,8 +15,12 @@
 
 namespace unetmi {
 
-constexpr int kTile = 16;                 // steps per tile of the forward kernels
+constexpr int kAlign = 16;                // chunks of the time axis start at multiples of this
 constexpr int kCh = 64;                   // channels per block
+
+// Steps per tile of the forward kernels: a tile's computation has to cover the next one's loads, and with few states a step
+// is short (16 x 1024 x 2048 bf16: 137 us for 4 and 140 for 8 states with 32 steps, 186 and 196 with 16; 16 states: 99 and 95).
+template <int S> constexpr int tile_steps() { return S <= 2 ? 32 : 16; }
 
 // steps between two saved states, = the steps the backward kernel keeps in registers
 template <int S> constexpr int mark_steps() { return S <= 2 ? 16 : S == 4 ? 8 : 4; }
@@ -201,7 +205,7 @@ enum ScanPass { kStates, kOutputs, kMarks };
 
 template <class T, int S, ScanPass PASS>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
-    constexpr int NP = 4 * S, MK = mark_steps<S>();
+    constexpr int NP = 4 * S, MK = mark_steps<S>(), kTile = tile_steps<S>();
     constexpr bool STATE_ONLY = PASS == kStates;
     __shared__ float lds_b[2][kTile * NP], lds_c[STATE_ONLY ? 1 : 2][STATE_ONLY ? 1 : kTile * NP];
     const Place p = place(a, blockIdx.z);
@@ -307,7 +311,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 // eight chunks: 125 us, vector units 90 % busy.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_bwd_state_kernel(ScanArgs a) {
-    constexpr int NP = 4 * S;
+    constexpr int NP = 4 * S, kTile = tile_steps<S>();
     __shared__ float lds_c[2][kTile * NP];
     const Place p = place(a, blockIdx.z);
     const int chunk = blockIdx.y + 1;                                 // nobody stands before the first chunk
@@ -680,8 +684,10 @@ struct ScanPlan {
 // Time is split where the blocks of the batch's channels alone do not fill the chip's 256 CUs: the first pass over the
 // chunks costs about 0.6 of the second, so it does not pay before (128 sequences of 501 steps, 512 blocks: 104 us in one
 // chunk, 35 + 94 us in two; 1 x 8192 steps x 2048 channels, 32 blocks: 99 + 64 us in 16 chunks, 90 + 60 in 32, 98 + 58 in
-// 64).  The backward kernel, two blocks a CU, gains from a split up to 384.  Sequences that end early (`ragged`) leave
-// their last chunks empty, and finer chunks even that out (8 x 2001 x 1280: 195 us in 3 chunks, 156 in 6, 122 in 21).
+// 64).  With up to 8 states, where a step is short and one wave a SIMD waits for its loads, a split still pays at 256 blocks
+// (8 x 2048 x 2048 x 4: 227 us in one chunk, 177 in four).  The backward kernel, two blocks a CU, gains from a split up to
+// 384 blocks.  Sequences that end early (`ragged`) leave their last chunks empty, and finer chunks even that out (8 x 2001 x
+// 1280: 195 us in 3 chunks, 156 in 6, 122 in 21).
 ScanPlan scan_plan(const UnetmiScanDesc& d, bool ragged, bool backward) {
     ScanPlan p;
     p.S = lane_states(d.state);
@@ -690,14 +696,14 @@ ScanPlan scan_plan(const UnetmiScanDesc& d, bool ragged, bool backward) {
     p.tpg = (Dg + kCh - 1) / kCh;
     const long long blocks = (long long)d.batch * d.groups * p.tpg;
     long long want = 1;
-    if (blocks > 0 && blocks < (backward ? 384 : 256)) want = ((ragged ? 4096 : 1024) + blocks - 1) / blocks;
+    if (blocks > 0 && blocks < (backward ? 384 : p.S <= 2 ? 320 : 256)) want = ((ragged ? 4096 : 1024) + blocks - 1) / blocks;
     const long long most = (d.length + 63) / 64;                      // chunks of at least 64 steps
     if (want > most) want = most;
     if (want > 64) want = 64;
     if (want < 1) want = 1;
     p.chunk = (int)((d.length + want - 1) / want);
-    p.chunk = (p.chunk + kTile - 1) / kTile * kTile;
-    if (p.chunk < kTile) p.chunk = kTile;
+    p.chunk = (p.chunk + kAlign - 1) / kAlign * kAlign;
+    if (p.chunk < kAlign) p.chunk = kAlign;
     p.nchunk = (d.length + p.chunk - 1) / p.chunk;
     if (p.nchunk < 1) p.nchunk = 1;
     const int mk = mark_steps_of(p.S);
@@ -716,12 +722,12 @@ int scan_check(const UnetmiScanDesc* d, const char* what) {
     if (d->channels > (1 << 22) || d->length > (1 << 28)) return api_fail(UNETMI_E_UNSUPPORTED, w + ": more than 2^22 channels or 2^28 steps");
     for (const int64_t* s : {d->x_stride, d->dt_stride, d->z_stride, d->dy_stride}) {
         if (s[0] < 0 || s[1] < 0) return api_fail(UNETMI_E_BAD_DESC, w + ": negative stride");
-        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^25 elements apart");
+        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^24 elements apart");
     }
     for (const int64_t* s : {d->b_stride, d->c_stride})
         if (s[0] < 0 || s[1] < 0 || s[2] < 0) return api_fail(UNETMI_E_BAD_DESC, w + ": negative stride");
     for (const int64_t* s : {d->b_stride, d->c_stride})
-        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^25 elements apart");
+        if (s[1] > UNETMI_SEQ_MAX_STEP) return api_fail(UNETMI_E_UNSUPPORTED, w + ": steps more than 2^24 elements apart");
     return UNETMI_OK;
 }
 
