@@ -4,6 +4,8 @@ leave.  Rounding counts: a state after m steps has taken two roundings a step an
 2^-24 of values whose sum of exponents bounds them), a sum over n terms at most n; hardware exponentials, reciprocals and
 the softplus series add a few tens."""
 
+import gc
+
 import pytest
 import torch
 
@@ -288,6 +290,30 @@ def test_selective_scan_at_the_ends_of_the_ranges(device):
         held(g, want["d_" + k], room["d_" + k], 4 * 64 + 2 * 16 + 96 + 400 + 64, "d " + k)
 
 
+@pytest.mark.parametrize("N", [3, 8, 16])
+def test_selective_scan_of_a_growing_state_that_starts_late(device, N):
+    """A > 0 over a split time axis: a state that is still zero stays zero where the decay of a whole chunk overflows."""
+    from unet_amd import ssm
+    L, ch = 512, 64
+    x, dy = rnd((1, L, ch), 1), rnd((1, L, ch), 2)
+    x[:, :-3] = 0
+    dy[:, 3:] = 0
+    p = dict(x=x, dt=torch.ones(1, L, ch), A=torch.full((ch, N), 2.0), B=rnd((1, L, 1, N), 3), C=rnd((1, L, 1, N), 4))
+    q = {k: v.to(device).requires_grad_() for k, v in p.items()}
+    y = ssm.selective_scan(**q, softplus=False)
+    grads = torch.autograd.grad(y, list(q.values()), dy.to(device))
+    want, room = (scan64(**p, softplus=False, dy=dy, magnitude=m) for m in (False, True))
+    held(y, want["y"], room["y"], 2 * L + N + 64, "y")
+    for k, g in zip(q, grads):
+        held(g, want["d_" + k], room["d_" + k], 5 * L + 2 * N + 96 + ch, "d " + k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,L,lengths", [(4, 330, [330, 0, 223]), (8, 289, None), (5, 1000, [1000, 511, 65])])
+def test_selective_scan_of_few_states_in_chunks(device, N, L, lengths, dtype):
+    scan_case(device, dtype, 3, L, 72, N, 1, True, True, True, True, True, lengths, False)
+
+
 def test_more_than_two_to_the_31_elements(device):
     """Sequences, caches and rows whose last elements lie beyond 2^31: the same bits as the last part on its own."""
     from unet_amd import norm, ssm
@@ -459,6 +485,37 @@ def test_block_gradients_in_a_graph(device):
         assert all(torch.equal(a, b) for a, b in zip(kept, eager)), [i for i, (a, b) in enumerate(zip(kept, eager)) if not torch.equal(a, b)]
 
 
+def test_a_captured_backward_beside_an_eager_graph(device):
+    """While an eager graph of the same leaves lives, their gradients belong to the default stream, which a capture cannot
+    wait for: the backward pass says so before it is tried.  Once that graph is gone the same capture works."""
+    from unet_amd import norm, ssm
+    w = rnd((64, 4), 1).to(device).requires_grad_()
+    A = (-0.1 - torch.rand(64, 8, generator=torch.Generator().manual_seed(6))).to(device).requires_grad_()
+    scale = rnd((64,), 2).to(device).requires_grad_()
+    x, dy = rnd((2, 40, 64), 3).to(device), rnd((2, 40, 64), 4).to(device)
+    bc = rnd((2, 40, 8), 5).to(device)
+    calls = [("causal_conv", lambda: ssm.causal_conv(x, w), w), ("selective_scan", lambda: ssm.selective_scan(x, x, A, bc, bc), A),
+             ("block_norm", lambda: norm.block_norm(x, residual=x, scale=scale), scale)]
+    for name, call, leaf in calls:
+        want, = torch.autograd.grad(call(), leaf, dy)
+        alive = call()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="eager graph on the default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(call(), leaf, dy)
+        torch.cuda.synchronize()
+        del alive
+        gc.collect()                                                   # the refused graph, which the exception's frames held
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(call(), leaf, dy)
+        for _ in range(3):
+            got.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want), name
+
+
 def test_tokens_in_a_graph(device):
     """A block's token step captured once and replayed over a growing stream, two graphs in turn on two caches, with eager
     work between: every token is the eager one, bit for bit."""
@@ -626,3 +683,8 @@ def test_refusals_on_the_device(device):
         norm.block_norm(torch.zeros(1, 8200, device=device), post_weight=torch.ones(8200, device=device))
     with pytest.raises(ValueError, match="one shape"):
         norm.block_norm(x, gate=x[:, :2])
+    with pytest.raises(ValueError, match="too long"):                  # one element each: nothing is allocated
+        ssm.causal_conv(x[:, :1, :1].expand(2 ** 32 + 1, 1, 1), torch.zeros(1, 4, device=device))
+    long = x[:, :1, :1].expand(1, 2 ** 32 + 1, 1)
+    with pytest.raises(ValueError, match="too long"):
+        ssm.selective_scan(long, long, A[:1], bc[:, :1].expand(1, 2 ** 32 + 1, 2), bc[:, :1].expand(1, 2 ** 32 + 1, 2))

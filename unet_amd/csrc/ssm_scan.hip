@@ -173,14 +173,13 @@ struct Shared {
     __device__ __forceinline__ Shared(const void* p, long long sb, long long st, long long sg, const Place& pl, int t0, int N)
         : base(static_cast<const T*>(p) + pl.b * sb + pl.g * sg + t0 * st), stride(st), row(threadIdx.x / NP) {
         const int n = threadIdx.x % NP;
-        off = n < N ? (row * (int)st + n) * (int)sizeof(T) : kOutside;
+        off = n < N && row < STEPS ? (row * (int)st + n) * (int)sizeof(T) : kOutside;
     }
     __device__ __forceinline__ void load(int dt, int left) {
         const auto rs = window(base + dt * stride);
 #pragma unroll
         for (int k = 0; k < E; ++k) {
-            const int i = row + k * ROWS;
-            v[k] = window_load<T>(rs, i < left && i < STEPS ? off : kOutside, k * ROWS * (int)stride * (int)sizeof(T));
+            v[k] = window_load<T>(rs, row + k * ROWS < left ? off : kOutside, k * ROWS * (int)stride * (int)sizeof(T));
         }
     }
     __device__ __forceinline__ void store(float* lds) const {
@@ -234,7 +233,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
             load_padded<S>(e, a.hend + row * NP, p.q);
             const float sd = a.sdt[row];
 #pragma unroll
-            for (int s = 0; s < S; ++s) h[s] = fmaf(exp2_hw(A2[s] * sd), h[s], e[s]);
+            for (int s = 0; s < S; ++s) h[s] = h[s] == 0.f ? e[s] : fmaf(exp2_hw(A2[s] * sd), h[s], e[s]);   // A > 0: 0, not 0 inf
         }
     }
     const OutColumn<T, kTile> out(a.y, a.D, (size_t)p.b * a.L + t0, p);
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs 
         load_padded<S>(e, a.hend + row * NP, p.q);
         const float sd = a.sdt[row];
 #pragma unroll
-        for (int s = 0; s < S; ++s) g[s] = fmaf(exp2_hw(A2[s] * sd), g[s], e[s]);
+        for (int s = 0; s < S; ++s) g[s] = g[s] == 0.f ? e[s] : fmaf(exp2_hw(A2[s] * sd), g[s], e[s]);
     }
     const size_t first = (size_t)p.b * a.L + t0;                      // row of the chunk's first step
     const OutColumn<T, MK> dx(a.dx, a.D, first, p), ddt(a.ddt, a.D, first, p), dz(a.dz, a.D, first, p);

@@ -9,6 +9,7 @@
 // allocator call by call (under graph capture: from the graph's own pool), never from a buffer that calls share.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -47,6 +48,12 @@ void check(int code, const char* what) {
     char text[512] = "";
     lib.last_error(text, sizeof text);
     TORCH_CHECK(false, what, " failed (", code, "): ", text);
+}
+
+// the library counts in 32 bits, and refuses what is larger than it takes itself
+int32_t count(int64_t n, const char* op) {
+    TORCH_CHECK_VALUE(n <= INT32_MAX, "unetmi::", op, ": an axis of ", n, " elements is too long");
+    return (int32_t)n;
 }
 
 int32_t kind(const Tensor& x, const char* op, int64_t axes) {
@@ -104,7 +111,7 @@ UnetmiSeqConvDesc conv_desc(const char* op, const Tensor& x, const Tensor& weigh
     dense(bias, "bias", op, at::kFloat, x, {D});
     dense(state, "state", op, x.scalar_type(), x, {B, K - 1, D});
     dense(lengths, "lengths", op, at::kInt, x, {B});
-    d.batch = B; d.length = x.size(1); d.channels = D; d.taps = K;
+    d.batch = count(B, op); d.length = count(x.size(1), op); d.channels = count(D, op); d.taps = count(K, op);
     d.act = silu ? UNETMI_ACT_SILU : UNETMI_ACT_NONE;
     return d;
 }
@@ -156,12 +163,14 @@ Tensor seq_conv_step(const Tensor& x0, const Tensor& weight, const Maybe& bias, 
     dense(bias, "bias", op, at::kFloat, x0, {D});
     dense(state, "state", op, x0.scalar_type(), x0, {state.size(0), K - 1, D});
     dense(slots, "slots", op, at::kInt, x0, {B});
+    const int32_t slot_count = count(state.size(0), op);
+    d.batch = count(B, op); d.length = 1; d.channels = count(D, op); d.taps = count(K, op);
     const Tensor x = rows(x0);
-    d.batch = B; d.length = 1; d.channels = D; d.taps = K; d.act = silu ? UNETMI_ACT_SILU : UNETMI_ACT_NONE;
+    d.act = silu ? UNETMI_ACT_SILU : UNETMI_ACT_NONE;
     d.x_stride[0] = x.stride(0);
     const c10::DeviceGuard guard(x.device());
     const Tensor y = empty(x.sizes(), x);
-    check(lib.conv_step(&d, ptr(x), f32(weight), f32(bias), i32(slots), state.size(0), ptr(state), ptr(y), stream_of(x)), "unetmi_seq_conv_step");
+    check(lib.conv_step(&d, ptr(x), f32(weight), f32(bias), i32(slots), slot_count, ptr(state), ptr(y), stream_of(x)), "unetmi_seq_conv_step");
     written(state);
     return y;
 }
@@ -190,10 +199,10 @@ struct ScanIn {
         dense(A, "A", op, at::kFloat, x0, {channels, N});
         dense(D, "D", op, at::kFloat, x0, {channels});
         dense(dt_bias, "dt_bias", op, at::kFloat, x0, {channels});
+        d.batch = count(x0.size(0), op); d.length = axes == 3 ? count(x0.size(1), op) : 1; d.channels = count(channels, op); d.state = count(N, op);
+        d.groups = grouped ? count(B0.size(axes - 1), op) : 1;
         x = rows(x0); dt = rows(dt0); B = rows(B0); C = rows(C0);
         if (z0) z = rows(*z0);
-        d.batch = x.size(0); d.length = axes == 3 ? x.size(1) : 1; d.channels = channels; d.state = N;
-        d.groups = grouped ? B.size(axes - 1) : 1;
         d.softplus = softplus;
         for (int64_t i = 0; i < axes - 1; ++i) {
             d.x_stride[i] = x.stride(i); d.dt_stride[i] = dt.stride(i); d.z_stride[i] = z ? z->stride(i) : 0;
@@ -268,9 +277,10 @@ Tensor ssm_scan_step(const Tensor& x0, const Tensor& dt0, const Tensor& A, const
     TORCH_CHECK_VALUE(state.dim() == 3, "unetmi::", op, ": state must be [slots, channels, state]");
     dense(state, "state", op, at::kFloat, x, {state.size(0), d.channels, d.state});
     dense(slots, "slots", op, at::kInt, x, {d.batch});
+    const int32_t slot_count = count(state.size(0), op);
     const c10::DeviceGuard guard(x.device());
     const Tensor y = empty(x.sizes(), x);
-    check(lib.scan_step(&d, ptr(x), ptr(in.dt), f32(A), ptr(in.B), ptr(in.C), f32(D), ptr(in.z), f32(dt_bias), i32(slots), state.size(0), f32(state),
+    check(lib.scan_step(&d, ptr(x), ptr(in.dt), f32(A), ptr(in.B), ptr(in.C), f32(D), ptr(in.z), f32(dt_bias), i32(slots), slot_count, f32(state),
                         ptr(y), stream_of(x)), "unetmi_ssm_scan_step");
     written(state);
     return y;
@@ -302,7 +312,7 @@ struct NormIn {
             residual = rows(*residual0);
             d.residual_stride = residual->stride(0);
         }
-        d.rows = shape[0]; d.channels = shape[1]; d.eps = eps; d.x_stride = x.stride(0);
+        d.rows = shape[0]; d.channels = count(shape[1], op); d.eps = eps; d.x_stride = x.stride(0);
         d.residual_dtype = residual_type == at::kBFloat16 ? UNETMI_DTYPE_BF16 : UNETMI_DTYPE_F32;
     }
 };
@@ -369,6 +379,21 @@ variable_list once(const char* what, variable_list gradients) {
     return (*node)(std::move(gradients));
 }
 
+// A captured backward pass cannot hand its gradients to a node that lives on the default stream, as the leaves' nodes do
+// while an eager graph of the same leaves is alive: waiting on that stream breaks the capture, and ends the process later.
+// Said here, before that wait.
+void joins_capture(const char* what) {
+    const auto here = c10::hip::getCurrentHIPStream();
+    if (here.id() == 0) return;                                       // the default stream is never captured
+    const auto node = torch::autograd::get_current_node();
+    if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const auto& edge : node->next_edges()) {
+        const auto stream = edge.function ? edge.function->stream() : std::nullopt;
+        TORCH_CHECK(!stream || stream->id() != 0, "unet_amd: the backward pass of ", what, " is being captured into a graph, but an input's gradient "
+                    "belongs to an eager graph on the default stream: free that graph (its outputs) before the capture, or run it on another stream");
+    }
+}
+
 template <class F>
 auto typed(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -388,6 +413,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;
+        joins_capture("causal_conv");
         const variable_list s = ctx->get_saved_variables();
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
         const Maybe dout = grads[1].defined() && grads[1].numel() ? Maybe(grads[1].contiguous()) : Maybe();
@@ -423,6 +449,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(12);
         if (!grads[0].defined() && !grads[1].defined()) return out;
+        joins_capture("selective_scan");
         const variable_list s = ctx->get_saved_variables();
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
         const Maybe dout = grads[1].defined() && grads[1].numel() ? Maybe(grads[1].contiguous()) : Maybe();
@@ -473,6 +500,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(7);
+        joins_capture("block_norm");
         const variable_list s = ctx->get_saved_variables();
         const Maybe d_out = grads[0].defined() ? Maybe(grads[0].contiguous()) : Maybe();
         const Maybe d_norm = s[4].defined() && grads[1].defined() ? Maybe(grads[1].contiguous()) : Maybe();

@@ -58,7 +58,7 @@ def causal_conv_step(x, state, weight, bias=None, act=True, slots=None):
 
 
 def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=None, lengths=None, return_state=False):
-    """x, dt, z [batch, length, channels], A [channels, N] (N <= 64; negative for a decaying state), B and C
+    """x, dt, z [batch, length, channels], A [channels, N] (N <= 64; finite, negative for a decaying state), B and C
     [batch, length, N] or [batch, length, groups, N], D and dt_bias [channels] -> y like x.
 
     softplus=False takes dt + dt_bias as the step sizes themselves.  state [batch, channels, N] fp32: where the recurrence
