@@ -612,6 +612,26 @@ def test_gradients_under_create_graph(device):
             g.sum().backward()
 
 
+def test_ops_under_dispatcher_checks(device):
+    """Schemas (what is written in place), autograd registration, shape inference, and the traced forward and backward with
+    symbolic sizes."""
+    B, L, C, N = 2, 40, 64, 8
+    r = lambda *s: rnd(s, 1).to(device)  # noqa: E731
+    g = lambda *s: r(*s).requires_grad_()  # noqa: E731
+    A = -torch.arange(1.0, N + 1).expand(C, N).contiguous().to(device)
+    for name, args in (
+            ("seq_conv", (g(B, L, C), g(C, 4), g(C), g(B, 3, C), None, True, True)),
+            ("seq_conv", (g(B, L, C), g(C, 4), None, None, None, False, False)),
+            ("seq_conv_step", (r(B, C), r(C, 4), None, r(B, 3, C), None, True)),
+            ("ssm_scan", (g(B, L, C), g(B, L, C), A.clone().requires_grad_(), g(B, L, N), g(B, L, N), g(C), g(B, L, C), g(C), g(B, C, N), None,
+                          True, True, False)),
+            ("ssm_scan", (g(B, L, C), g(B, L, C), A, g(B, L, 2, N), g(B, L, 2, N), None, None, None, None, None, True, False, False)),
+            ("ssm_scan_step", (r(B, C), r(B, C), A, r(B, N), r(B, N), None, None, None, r(B, C, N), None, True)),
+            ("block_norm", (g(5, C), g(5, C), g(C), g(5, C), g(C), g(C), 1e-6)),
+            ("block_norm", (g(5, C), None, g(C), None, None, None, 1e-6))):
+        torch.library.opcheck(getattr(torch.ops.unetmi, name).default, args)
+
+
 def test_leaves_that_want_no_gradient(device):
     """Only some inputs want gradients, optional ones among them given and not: each gets its own."""
     from unet_amd import norm, ssm

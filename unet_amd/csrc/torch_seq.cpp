@@ -416,7 +416,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
         joins_capture("causal_conv");
         const variable_list s = ctx->get_saved_variables();
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
-        const Maybe dout = grads[1].defined() && grads[1].numel() ? Maybe(grads[1].contiguous()) : Maybe();
+        const Maybe dout = grads[1].defined() && grads[1].dim() == 3 ? Maybe(grads[1].contiguous()) : Maybe();
         static auto op = typed<decltype(seq_conv_bwd)>("unetmi::seq_conv_bwd");
         auto [dx, dw, db, ds] = op.call(s[0], s[1], maybe(s[2]), maybe(s[3]), maybe(s[4]), ctx->saved_data["silu"].toBool(), dy, dout);
         Wanted wanted{ctx};
@@ -452,7 +452,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
         joins_capture("selective_scan");
         const variable_list s = ctx->get_saved_variables();
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
-        const Maybe dout = grads[1].defined() && grads[1].numel() ? Maybe(grads[1].contiguous()) : Maybe();
+        const Maybe dout = grads[1].defined() && grads[1].dim() == 3 ? Maybe(grads[1].contiguous()) : Maybe();
         Wanted wanted{ctx};
         bool want[9];
         for (int i = 0; i < 5; ++i) want[i] = wanted.next();
