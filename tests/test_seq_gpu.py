@@ -615,6 +615,7 @@ def test_gradients_under_create_graph(device):
 def test_ops_under_dispatcher_checks(device):
     """Schemas (what is written in place), autograd registration, shape inference, and the traced forward and backward with
     symbolic sizes."""
+    import unet_amd  # noqa: F401
     B, L, C, N = 2, 40, 64, 8
     r = lambda *s: rnd(s, 1).to(device)  # noqa: E731
     g = lambda *s: r(*s).requires_grad_()  # noqa: E731
