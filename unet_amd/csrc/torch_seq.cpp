@@ -394,6 +394,16 @@ void joins_capture(const char* what) {
     }
 }
 
+// whether autograd records a call on these tensors
+bool recorded(std::initializer_list<const Tensor*> given, std::initializer_list<const Maybe*> optional) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor* t : given)
+        if (t->requires_grad()) return true;
+    for (const Maybe* t : optional)
+        if (*t && (*t)->requires_grad()) return true;
+    return false;
+}
+
 template <class F>
 auto typed(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -429,6 +439,11 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
 };
 std::tuple<Tensor, Tensor> seq_conv_autograd(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& state, const Maybe& lengths,
                                              bool silu, bool want_state) {
+    if (!recorded({&x, &weight}, {&bias, &state})) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static auto op = typed<decltype(seq_conv)>("unetmi::seq_conv");
+        return op.call(x, weight, bias, state, lengths, silu, want_state);
+    }
     const variable_list r = ConvNode::apply(x, weight, bias, state, lengths, silu, want_state);
     return {r[0], r[1]};
 }
@@ -471,12 +486,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
 std::tuple<Tensor, Tensor, Tensor> ssm_scan_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                                                      const Maybe& D, const Maybe& z, const Maybe& dt_bias, const Maybe& state, const Maybe& lengths,
                                                      bool softplus, bool want_state, bool want_marks) {
-    bool needed = false;
-    if (at::GradMode::is_enabled()) {
-        for (const Tensor* t : {&x, &dt, &A, &B, &C}) needed |= t->requires_grad();
-        for (const Maybe* t : {&D, &z, &dt_bias, &state}) needed |= *t && (*t)->requires_grad();
-    }
-    if (!needed) {                                                    // no node: and no states saved for one
+    if (!recorded({&x, &dt, &A, &B, &C}, {&D, &z, &dt_bias, &state})) {       // no node, and no states saved for one
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(ssm_scan)>("unetmi::ssm_scan");
         return op.call(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state, want_marks);
@@ -521,6 +531,11 @@ struct NormNode : torch::autograd::Function<NormNode> {
 };
 std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
                                                const Maybe& pre, double eps) {
+    if (!recorded({&x}, {&gate, &post, &residual, &scale, &pre})) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        static auto op = typed<decltype(block_norm)>("unetmi::block_norm");
+        return op.call(x, gate, post, residual, scale, pre, eps);
+    }
     const variable_list r = NormNode::apply(x, gate, post, residual, scale, pre, eps);
     return {r[0], r[1]};
 }
