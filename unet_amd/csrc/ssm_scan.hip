@@ -619,9 +619,9 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
 }
 
 // One token of every row; state [slots, D, N] is read and written once: 8N bytes a channel against 7N operations, HBM
-// bound: 256 rows x 2048 channels x 16 states in 18.4 us (3.9 TB/s; 39 with a block per 64 channels and single loads); one
-// row of 1280 channels in 4.  A block takes a row's blocks of 64 channels in turn (of one group: B and C are loaded once), so that the check of
-// the row's slot against the rows before it is paid once for several of them.
+// bound: 256 rows x 2048 channels x 16 states in 17 us (4.2 TB/s; 39 with a block per 64 channels and single loads); one row
+// of 1280 channels in 4.  A block takes a row's blocks of 64 channels in turn (of one group: B and C are loaded once), so that
+// the check of the row's slot against the rows before it is paid once for several of them.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a, int parts, const int* __restrict__ slots, int nslots, float* __restrict__ state) {
     const int row = blockIdx.y, g = blockIdx.x / parts, part = blockIdx.x - g * parts;
@@ -799,8 +799,8 @@ struct RunScanBwd {
 template <class T, int S>
 struct RunScanStep {
     static int run(const UnetmiScanDesc& d, const ScanPlan& p, const ScanArgs& a, const int* slots, int nslots, float* state, hipStream_t s) {
-        // about four blocks a CU, as long as that many rows and channels are there
-        long long parts = (1024 + (long long)d.batch * d.groups - 1) / ((long long)d.batch * d.groups);
+        // about eight blocks a CU, as long as that many rows and channels are there (256 x 2048 x 16: 17.1 us, four 19.6, sixteen 20.2)
+        long long parts = (2048 + (long long)d.batch * d.groups - 1) / ((long long)d.batch * d.groups);
         if (parts > p.tpg) parts = p.tpg;
         hipLaunchKernelGGL((scan_step_kernel<T, S>), dim3(d.groups * (int)parts, d.batch), dim3(256), 0, s, a, (int)parts, slots, nslots, state);
         return launched("ssm_scan_step");
