@@ -431,6 +431,90 @@ def test_empty_calls(device):
     assert norm.block_norm(e(0, 8), post_weight=torch.ones(8, device=device)).shape == (0, 8)
 
 
+def test_gradients_of_empty_calls(device):
+    """No step or no sequence: parameters get zeros, a state's gradient goes straight through."""
+    from unet_amd import norm, ssm
+    for B, L in ((2, 0), (0, 5), (0, 0)):
+        x = torch.zeros(B, L, 8, device=device, requires_grad=True)
+        bc = torch.zeros(B, L, 4, device=device, requires_grad=True)
+        A = -torch.ones(8, 4, device=device)
+        A.requires_grad_()
+        state, before = rnd((B, 8, 4), 1).to(device).requires_grad_(), rnd((B, 2, 8), 2).to(device).requires_grad_()
+        w, b = rnd((8, 3), 3).to(device).requires_grad_(), rnd((8,), 4).to(device).requires_grad_()
+        ds, dc = rnd((B, 8, 4), 5).to(device), rnd((B, 2, 8), 6).to(device)
+        y, s = ssm.selective_scan(x, x, A, bc, bc, D=b, z=x, dt_bias=b, state=state, return_state=True)
+        gx, gA, gb, gs = torch.autograd.grad((y, s), (x, A, b, state), (torch.zeros_like(y), ds))
+        assert gx.shape == x.shape and torch.equal(gs, ds) and not gA.any() and not gb.any()
+        y, s = ssm.causal_conv(x, w, b, state=before, return_state=True)
+        gx, gw, gb, gs = torch.autograd.grad((y, s), (x, w, b, before), (torch.zeros_like(y), dc))
+        assert gx.shape == x.shape and torch.equal(gs, dc) and not gw.any() and not gb.any()
+    x = torch.zeros(0, 8, device=device, requires_grad=True)
+    r, n = norm.block_norm(x, gate=x, post_weight=b, residual=x, scale=b, pre_weight=b)
+    gx, gb = torch.autograd.grad((r, n), (x, b), (torch.zeros_like(r), torch.zeros_like(n)))
+    assert gx.shape == x.shape and not gb.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_inputs_in_other_orders(device, dtype):
+    """Channels-first tensors seen through a transpose, inputs broadcast over the batch or the groups, gradients that arrive
+    expanded: what the same values give when dense, bit for bit, and a broadcast input's gradient is the sum over its copies."""
+    from unet_amd import norm, ssm
+    B, L, C, N, G = 3, 45, 48, 5, 4
+    A = (-torch.rand((C, N), generator=torch.Generator().manual_seed(1)) - 0.1).to(device)
+    w, one = rnd((C, 4), 2).to(device), rnd((C,), 3).to(device)
+    x = rnd((B, C, L), 4, dtype).to(device).transpose(1, 2)
+    dt = rnd((1, L, C), 5, dtype).to(device).expand(B, L, C)
+    bm = rnd((B, L, 1, N), 6, dtype).to(device).expand(B, L, G, N)
+    cm = rnd((B, N, L, G), 7, dtype).to(device).permute(0, 2, 3, 1)
+    z = rnd((B, L, 1), 8, dtype).to(device).expand(B, L, C)
+    dy = rnd((1, 1, C), 9, dtype).to(device).expand(B, L, C)
+
+    def both(call, *tensors):
+        out = []
+        for dense in (False, True):
+            leaves = [(t.contiguous() if dense else t.detach()).requires_grad_() for t in tensors]
+            y = call(*leaves)
+            out.append([y] + list(torch.autograd.grad(y, leaves, dy.reshape(y.shape) if not dense else dy.contiguous().reshape(y.shape))))
+        assert all(torch.equal(a, b) for a, b in zip(*out))
+
+    both(lambda x, dt, bm, cm, z: ssm.selective_scan(x, dt, A, bm, cm, D=one, z=z, dt_bias=one), x, dt, bm, cm, z)
+    both(lambda x: ssm.causal_conv(x, w, one), x)
+    both(lambda z: ssm.causal_conv(z, w, one), z)
+    both(lambda x, z: norm.block_norm(x, gate=z, post_weight=one), x, z)
+    both(lambda x, z: norm.block_norm(x, residual=z, pre_weight=one)[1], x, z)
+    narrow = rnd((B, L, 1, N), 6, dtype).to(device).requires_grad_()
+    wide = narrow.detach().expand(B, L, G, N).contiguous().requires_grad_()
+    g, = torch.autograd.grad(ssm.selective_scan(x, dt, A, narrow.expand(B, L, G, N), cm), narrow, dy)
+    h, = torch.autograd.grad(ssm.selective_scan(x, dt, A, wide, cm), wide, dy)
+    assert torch.equal(g, h.sum(2, keepdim=True))
+    # tokens
+    state, cache = rnd((B, C, N), 10).to(device), rnd((B, 3, C), 11, dtype).to(device)
+    for t in (0, L - 1):
+        s, c = state.clone(), cache.clone()
+        a = ssm.selective_scan_step(x[:, t], dt[:, t], A, bm[:, t], cm[:, t], state, z=z[:, t])
+        b = ssm.selective_scan_step(*(v[:, t].contiguous() for v in (x, dt)), A, bm[:, t].contiguous(), cm[:, t].contiguous(), s, z=z[:, t].contiguous())
+        assert torch.equal(a, b) and torch.equal(s, state)
+        assert torch.equal(ssm.causal_conv_step(x[:, t], cache, w), ssm.causal_conv_step(x[:, t].contiguous(), c, w)) and torch.equal(c, cache)
+
+
+def test_inference_mode(device):
+    """Caches made inside and outside of inference mode."""
+    from unet_amd import norm, ssm
+    x = rnd((2, 6, 16), 1).to(device)
+    w, A, bc = rnd((16, 4), 2).to(device), -torch.ones(16, 4, device=device), rnd((2, 6, 4), 3).to(device)
+    want, state = ssm.selective_scan(x, x, A, bc, bc, return_state=True)
+    u, before = ssm.causal_conv(x, w, return_state=True)
+    outside = torch.zeros(2, 16, 4, device=device), torch.zeros(2, 3, 16, device=device)
+    with torch.inference_mode():
+        for s, c in (outside, (torch.zeros(2, 16, 4, device=device), torch.zeros(2, 3, 16, device=device))):
+            for t in range(6):
+                y = ssm.selective_scan_step(x[:, t], x[:, t], A, bc[:, t], bc[:, t], s)
+                v = ssm.causal_conv_step(x[:, t], c, w)
+            assert torch.allclose(y, want[:, -1], rtol=1e-4, atol=1e-5) and torch.allclose(s, state, rtol=1e-4, atol=1e-5)
+            assert torch.equal(c, before) and torch.allclose(v, u[:, -1], rtol=1e-5, atol=1e-6)
+        assert torch.equal(norm.block_norm(x, gate=x), norm.block_norm(x.clone(), gate=x.clone()))
+
+
 def block(p, x):
     """A state space block as a program has it: norm, projections, conv, scan, gated norm, projection, residual."""
     from unet_amd import norm, ssm

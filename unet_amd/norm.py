@@ -17,7 +17,7 @@ def block_norm(x, gate=None, post_weight=None, residual=None, scale=None, pre_we
     """x [..., channels] (channels <= 8192) -> p; with a residual -> r; with a residual and pre_weight -> (r, n).
 
     Every part is optional: without a gate u = x, without post_weight p = u, without a scale r = residual + p.  scale and the
-    weights are fp32 [channels]; scale may also be a single value.  x and gate are fp32 or bfloat16; the residual stream is of
+    weights are fp32 [channels]; scale may also be a tensor of one value.  x and gate are fp32 or bfloat16; the residual stream is of
     their type or fp32, and r is what the stream becomes.  Differentiable (once) in every tensor."""
     if residual is None and (scale is not None or pre_weight is not None):
         raise ValueError("unet_amd.norm: scale and pre_weight belong to a residual stream")
