@@ -125,11 +125,9 @@ def scan64(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, state=No
     return out
 
 
-def norm64(x, gate, post, residual, scale, pre, eps, d_out=None, d_norm=None, magnitude=False, stream=None):
-    """dict(p or r, n) and, with gradients given, dict(d_x, d_gate, d_post, d_residual, d_scale, d_pre).  stream: the r that
-    the gradients go by (the stored one), else the computed one."""
-    x, gate, post, residual, scale, pre, d_out, d_norm, stream = (
-        f64(t) for t in (x, gate, post, residual, scale, pre, d_out, d_norm, stream))
+def norm64(x, gate, post, residual, scale, pre, eps, d_out=None, d_norm=None, magnitude=False):
+    """dict(p or r, n) and, with gradients given, dict(d_x, d_gate, d_post, d_residual, d_scale, d_pre)."""
+    x, gate, post, residual, scale, pre, d_out, d_norm = (f64(t) for t in (x, gate, post, residual, scale, pre, d_out, d_norm))
     mag = (lambda t: t.abs()) if magnitude else (lambda t: t)
     u = mag(x)
     slope = None
@@ -159,9 +157,7 @@ def norm64(x, gate, post, residual, scale, pre, eps, d_out=None, d_norm=None, ma
     if residual is not None:
         d_r = d_p
         if pre is not None and d_norm is not None:
-            rr = plain_r if stream is None else stream
-            inv = torch.rsqrt(rr.pow(2).mean(-1, keepdim=True) + eps)
-            rr = mag(rr)
+            inv, rr = inv_r, r
             g = mag(d_norm) * mag(pre)
             out["d_pre"] = (mag(d_norm) * rr * inv).sum(0)
             d_r = d_r + inv * (g + sign * rr * inv * inv * (g * rr).mean(-1, keepdim=True))

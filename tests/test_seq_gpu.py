@@ -385,8 +385,8 @@ def test_block_norm(device, rows, D, gate, post, residual, scale, pre, xt, rt):
         leaves = {k: (put(v) if v.dim() == 2 else v.to(device)).requires_grad_() for k, v in zip(names, t) if v is not None}
         out = norm.block_norm(**leaves, eps=eps)
         out = out if pre else (out,)
-        want = norm64(*t, eps, d_out, d_n, stream=out[0] if pre else None)
-        room = norm64(*t, eps, d_out, d_n, magnitude=True, stream=out[0] if pre else None)
+        want = norm64(*t, eps, d_out, d_n)
+        room = norm64(*t, eps, d_out, d_n, magnitude=True)
         # a mean over a row: 8 terms a thread, 6 exchanges, 16 waves; its root halves the error, then a few products
         held(out[0], want["r" if residual else "p"], room["r" if residual else "p"], 64, "r")
         if pre:

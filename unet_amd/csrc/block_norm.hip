@@ -16,7 +16,7 @@ namespace unetmi {
 struct NormArgs {
     const void *x, *gate;                 // gate may be null
     const float *post, *scale, *pre;      // null: that part is left out (scale: 1)
-    const void* residual;                 // forward: the stream; backward: its new value r
+    const void* residual;
     long long xs, gs, rs;                 // elements between rows
     long long rows;
     int D;
@@ -142,7 +142,8 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
 //     dresidual = dr,  dscale = sum dr p,  dp = scale dr            (without a residual dp = d_r)
 //     du = e (q - u e^2 mean(q u)),  q = dp w_post                  dw_post = sum dp u e
 //     dx = du silu(gate),  dgate = du x silu'(gate)
-// f and e are computed again from the rows (they are read anyway); r is the stream as it was stored.
+// All of p, r, e and f are computed again from the inputs' rows, which are read anyway: a stream stored in 16 bits would leave
+// its rounding in the weights' gradients (2e-3 of dscale and dw_pre over a few rows).
 template <class T, class RT, int E>
 __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
     constexpr int V = kVector<T>;
@@ -163,7 +164,7 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < E; ++i) { u[i] = x[i]; g[i] = 0.f; }
         if (a.d_r) {
-            if (a.residual || a.dres) load_row<RT, V, E>(g, a.d_r, row * a.D, a.D, col, width);
+            if (a.dres) load_row<RT, V, E>(g, a.d_r, row * a.D, a.D, col, width);
             else load_row<T, V, E>(g, a.d_r, row * a.D, a.D, col, width);
         }
         if (a.gate) {
@@ -171,23 +172,29 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < E; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
         }
-        float s[3] = {0.f, 0.f, 0.f};
         const bool with_pre = a.pre && a.d_n;
         if (with_pre) {
             load_row<RT, V, E>(r, a.residual, row * a.rs, a.D, col, width);
             load_row<T, V, E>(dn, a.d_n, row * a.D, a.D, col, width);
+        }
+        float e = 1.f;
+        if (a.post) {
+            float s[1] = {0.f};
+#pragma unroll
+            for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
+            sum(s);
+            e = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
+        }
+        if (with_pre) {
+            float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                s[1] = fmaf(r[i], r[i], s[1]);
-                s[2] = fmaf(dn[i] * pre[i], r[i], s[2]);
+                r[i] = fmaf(scale[i] * post[i], u[i] * e, r[i]);
+                s[0] = fmaf(r[i], r[i], s[0]);
+                s[1] = fmaf(dn[i] * pre[i], r[i], s[1]);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
-        if (with_pre || a.post) sum(s);
-        const float e = a.post ? __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps)) : 1.f;
-        if (with_pre) {
-            const float f = __builtin_amdgcn_rsqf(fmaf(s[1], inv_d, a.eps)), m = f * f * s[2] * inv_d;
+            sum(s);
+            const float f = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps)), m = f * f * s[1] * inv_d;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
                 d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
@@ -324,17 +331,17 @@ size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d) {
     return (size_t)p.blocks * p.per_block * 3 * d->channels * sizeof(float);
 }
 
-int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* stream_out,
+int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
                           const float* scale, const float* pre_weight, const void* d_out, const void* d_norm, void* dx, void* dgate,
                           void* dresidual, float* dweights, void* ws, size_t ws_bytes, void* stream) {
     const int rc = norm_check(d, "block_norm_bwd");
     if (rc != UNETMI_OK) return rc;
     if (d->rows == 0) return api_fail(UNETMI_E_BAD_DESC, "block_norm_bwd: no rows");
-    if (!x || !dx || !dweights || !ws || (gate && !dgate) || (pre_weight && d_norm && !stream_out))
+    if (!x || !dx || !dweights || !ws || (gate && !dgate) || (pre_weight && d_norm && !residual))
         return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: null tensor pointer");
     if (!dresidual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: scale and pre_weight belong to a residual stream");
     if (ws_bytes < unetmi_block_norm_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: workspace too small");
-    NormArgs a = norm_args(*d, x, gate, post_weight, stream_out, scale, pre_weight);
+    NormArgs a = norm_args(*d, x, gate, post_weight, residual, scale, pre_weight);
     a.d_r = d_out; a.d_n = d_norm; a.dx = dx; a.dgate = dgate; a.dres = dresidual;
     a.partial = static_cast<float*>(ws);
     const NormPlan p = norm_plan(*d, bwd_blocks(*d));

@@ -332,12 +332,12 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& x0, const Maybe& gate, const
 }
 
 // (dx, dgate or empty, dresidual or empty, [dpost_weight, dscale, dpre_weight])
-std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_bwd(const Tensor& x0, const Maybe& gate, const Maybe& post, const Maybe& stream, const Maybe& scale,
+std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_bwd(const Tensor& x0, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
                                                           const Maybe& pre, double eps, const Maybe& d_out, const Maybe& d_norm, bool has_residual,
                                                           bool residual_f32) {
     const char* op = "block_norm_bwd";
     const at::ScalarType rtype = residual_f32 ? at::kFloat : x0.scalar_type();
-    const NormIn in(op, x0, gate, post, stream, scale, pre, eps, rtype);
+    const NormIn in(op, x0, gate, post, residual, scale, pre, eps, rtype);
     const Tensor& x = in.x;
     dense(d_out, "d_out", op, has_residual ? rtype : x.scalar_type(), x, x.sizes());
     dense(d_norm, "d_norm", op, x.scalar_type(), x, x.sizes());
@@ -501,7 +501,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(block_norm)>("unetmi::block_norm");
         auto [out, out_n] = op.call(x, gate, post, residual, scale, pre, eps);
-        ctx->save_for_backward({x, value(gate), value(post), value(scale), value(pre), pre ? out : Tensor()});
+        ctx->save_for_backward({x, value(gate), value(post), value(scale), value(pre), pre ? *residual : Tensor()});
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["residual"] = residual.has_value();
         ctx->saved_data["f32"] = residual && residual->scalar_type() == at::kFloat;
@@ -581,7 +581,7 @@ TORCH_LIBRARY_FRAGMENT(unetmi, m) {
           "Tensor? slots, bool softplus) -> Tensor");
     m.def("block_norm(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? residual, Tensor? scale, Tensor? pre_weight, float eps) "
           "-> (Tensor, Tensor)");
-    m.def("block_norm_bwd(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? stream, Tensor? scale, Tensor? pre_weight, float eps, "
+    m.def("block_norm_bwd(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? residual, Tensor? scale, Tensor? pre_weight, float eps, "
           "Tensor? d_out, Tensor? d_norm, bool has_residual, bool residual_f32) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(unetmi, CUDA, m) {                                 // ROCm tensors dispatch here

@@ -78,7 +78,7 @@ def _(x, gate, post_weight, residual, scale, pre_weight, eps):
 
 
 @torch.library.register_fake("unetmi::block_norm_bwd")
-def _(x, gate, post_weight, stream, scale, pre_weight, eps, d_out, d_norm, has_residual, residual_f32):
+def _(x, gate, post_weight, residual, scale, pre_weight, eps, d_out, d_norm, has_residual, residual_f32):
     return (x.new_empty(x.shape), x.new_empty((0,) if gate is None else x.shape),
             x.new_empty(x.shape if has_residual else (0,), dtype=torch.float32 if residual_f32 else x.dtype),
             x.new_empty((3, x.shape[1]), dtype=torch.float32))
