@@ -620,14 +620,14 @@ typedef struct UnetmiNormDesc {
 } UnetmiNormDesc;
 
 int unetmi_block_norm_fwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
-                          const float* scale, const float* pre_weight, void* out, void* out_norm, void* stream);
+                          const float* scale, const float* pre_weight, void* out, void* out_norm, float* stats, void* stream);
 
-/* Gradients.  residual is needed with pre_weight and d_norm only; d_out / d_norm:
- * the gradients of r (or p) and n, NULL for zero.  dresidual must be given where there was a residual.  dweights: one buffer
+/* Gradients.  stats: [rows, 2] that the forward call filled (NULL there in inference; the backward call needs it with
+ * post_weight or pre_weight).  residual is needed with pre_weight and d_norm only; d_out / d_norm: the gradients of r (or p) and n, NULL for zero.  dresidual must be given where there was a residual.  dweights: one buffer
  * [3, channels]: post_weight, scale, pre_weight. */
 size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d);
 int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
-                          const float* scale, const float* pre_weight, const void* d_out, const void* d_norm, void* dx, void* dgate,
+                          const float* scale, const float* pre_weight, const float* stats, const void* d_out, const void* d_norm, void* dx, void* dgate,
                           void* dresidual, float* dweights, void* ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -33,9 +33,10 @@ def test_sequence_ops_infer_shapes():
         assert [t.dtype for t in out] == [t.dtype for t in (x, x, A, B, B, c, x, c, h)]
         assert ops.ssm_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], c, None, c, h, None, True).shape == (2, 24)
         rows, r = x.reshape(-1, 24), torch.empty(74, 24)
-        out, n = ops.block_norm(rows, rows, c, r, c, c, 1e-6)
+        out, n, stats = ops.block_norm(rows, rows, c, r, c, c, 1e-6, True)
+        assert stats.shape == (rows.shape[0], 2) and stats.dtype == torch.float32
         assert out.shape == n.shape == rows.shape and out.dtype == torch.float32 and n.dtype == torch.bfloat16
-        dx, dg, dr, dw = ops.block_norm_bwd(rows, rows, c, r, c, c, 1e-6, r, rows, True, True)
+        dx, dg, dr, dw = ops.block_norm_bwd(rows, rows, c, r, c, c, 1e-6, stats, r, rows, True, True)
         assert dx.shape == dg.shape == dr.shape == rows.shape and dr.dtype == torch.float32 and dw.shape == (3, 24)
 
 
@@ -100,15 +101,16 @@ def test_c_entry_points_refuse():
     refused(lib.unetmi_ssm_scan_bwd(ref(scan(batch=0)), *[p] * 22, 0, None), _lib.E_BAD_DESC, "empty")
     refused(lib.unetmi_ssm_scan_step(ref(scan(batch=2)), *[p] * 8, None, 1, p, p, None), _lib.E_BAD_ARG, "slots")
 
-    fwd = lambda d, *a: lib.unetmi_block_norm_fwd(ref(d), *(a or [None] * 8), None)  # noqa: E731
+    fwd = lambda d, *a: lib.unetmi_block_norm_fwd(ref(d), *(a or [None] * 9), None)  # noqa: E731
     refused(fwd(norm()), _lib.E_BAD_ARG, "null")
     refused(fwd(norm(channels=8193)), _lib.E_UNSUPPORTED, "8192")
     refused(fwd(norm(dtype=1, residual_dtype=2)), _lib.E_UNSUPPORTED, "residual")
     refused(fwd(norm(eps=-1.0)), _lib.E_BAD_DESC, "eps")
     refused(fwd(norm(eps=float("nan"))), _lib.E_BAD_DESC, "eps")
-    refused(fwd(norm(), p, None, None, None, p, None, p, None), _lib.E_BAD_ARG, "residual")
-    refused(lib.unetmi_block_norm_bwd(ref(norm()), *[p] * 13, 0, None), _lib.E_BAD_ARG, "workspace")
-    refused(lib.unetmi_block_norm_bwd(ref(norm(rows=0)), *[p] * 13, 0, None), _lib.E_BAD_DESC, "rows")
+    refused(fwd(norm(), p, None, None, None, p, None, p, None, None), _lib.E_BAD_ARG, "residual")
+    refused(lib.unetmi_block_norm_bwd(ref(norm()), *[p] * 14, 0, None), _lib.E_BAD_ARG, "workspace")
+    refused(lib.unetmi_block_norm_bwd(ref(norm()), *[p] * 6, None, *[p] * 7, 1 << 30, None), _lib.E_BAD_ARG, "null")     # no stats
+    refused(lib.unetmi_block_norm_bwd(ref(norm(rows=0)), *[p] * 14, 0, None), _lib.E_BAD_DESC, "rows")
 
 
 def test_cpu_tensors_have_no_kernel():

@@ -712,8 +712,8 @@ def test_ops_under_dispatcher_checks(device):
                           True, True, False)),
             ("ssm_scan", (g(B, L, C), g(B, L, C), A, g(B, L, 2, N), g(B, L, 2, N), None, None, None, None, None, True, False, False)),
             ("ssm_scan_step", (r(B, C), r(B, C), A, r(B, N), r(B, N), None, None, None, r(B, C, N), None, True)),
-            ("block_norm", (g(5, C), g(5, C), g(C), g(5, C), g(C), g(C), 1e-6)),
-            ("block_norm", (g(5, C), None, g(C), None, None, None, 1e-6))):
+            ("block_norm", (g(5, C), g(5, C), g(C), g(5, C), g(C), g(C), 1e-6, False)),
+            ("block_norm", (g(5, C), None, g(C), None, None, None, 1e-6, False))):
         torch.library.opcheck(getattr(torch.ops.unetmi, name).default, args)
 
 

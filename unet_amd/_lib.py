@@ -241,8 +241,8 @@ def _load():
     lib.unetmi_ssm_scan_fwd.argtypes = [scan] + [vp] * 14 + [sz, vp]
     lib.unetmi_ssm_scan_bwd.argtypes = [scan] + [vp] * 22 + [sz, vp]
     lib.unetmi_ssm_scan_step.argtypes = [scan] + [vp] * 9 + [ci] + [vp] * 3
-    lib.unetmi_block_norm_fwd.argtypes = [norm] + [vp] * 9
-    lib.unetmi_block_norm_bwd.argtypes = [norm] + [vp] * 13 + [sz, vp]
+    lib.unetmi_block_norm_fwd.argtypes = [norm] + [vp] * 10
+    lib.unetmi_block_norm_bwd.argtypes = [norm] + [vp] * 14 + [sz, vp]
     for f in (lib.unetmi_seq_conv_fwd, lib.unetmi_seq_conv_bwd, lib.unetmi_seq_conv_step, lib.unetmi_ssm_scan_fwd, lib.unetmi_ssm_scan_bwd,
               lib.unetmi_ssm_scan_step, lib.unetmi_block_norm_fwd, lib.unetmi_block_norm_bwd):
         f.restype = ctypes.c_int

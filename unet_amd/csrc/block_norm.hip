@@ -22,6 +22,7 @@ struct NormArgs {
     int D;
     float eps;
     void *out_r, *out_n;                  // r (or p without a residual), n
+    float* stats;                         // [rows, 2]: 1 / rms(u), 1 / rms(r); null in inference
     // backward
     const void *d_r, *d_n;                // null: zero
     void *dx, *dgate, *dres;
@@ -114,6 +115,7 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
             for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
             sum(s);
             const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
+            if (a.stats && col == 0) a.stats[2 * row] = inv;
 #pragma unroll
             for (int i = 0; i < E; ++i) u[i] *= inv * post[i];
         }
@@ -130,6 +132,7 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
             for (int i = 0; i < E; ++i) s[0] = fmaf(r[i], r[i], s[0]);
             sum(s);
             const float inv = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
+            if (a.stats && col == 0) a.stats[2 * row + 1] = inv;
 #pragma unroll
             for (int i = 0; i < E; ++i) r[i] *= inv * pre[i];
             store_row<T, V, E>(r, a.out_n, row * a.D, a.D, col, width);
@@ -137,13 +140,15 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
     }
 }
 
-// Backward.  With f = 1 / rms(r), e = 1 / rms(u):
+// Backward.  With f = 1 / rms(r), e = 1 / rms(u) as the forward call saved them:
 //     dr = d_r + f (g - r f^2 mean(g r)),  g = d_n w_pre          dw_pre = sum_rows d_n r f
 //     dresidual = dr,  dscale = sum dr p,  dp = scale dr            (without a residual dp = d_r)
 //     du = e (q - u e^2 mean(q u)),  q = dp w_post                  dw_post = sum dp u e
 //     dx = du silu(gate),  dgate = du x silu'(gate)
-// All of p, r, e and f are computed again from the inputs' rows, which are read anyway: a stream stored in 16 bits would leave
-// its rounding in the weights' gradients (2e-3 of dscale and dw_pre over a few rows).
+// With w = scale w_post the second mean is linear in the first one, sum(q u) = sum(w u (d_r + f g)) - f^3 mean(g r) sum(w u r),
+// so the three sums are taken together and a row waits once (16032 x 1285 fp32: 175 us with e, f and the means one after the
+// other).  r is computed again from the residual, which has to be read anyway: a stream stored in 16 bits would leave its
+// rounding in the weights' gradients (2e-3 of dscale and dw_pre over a few rows).
 template <class T, class RT, int E>
 __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
     constexpr int V = kVector<T>;
@@ -157,70 +162,55 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
     if (a.scale) load_row<float, V, E>(scale, a.scale, 0, a.D, col, width);
     if (a.pre) load_row<float, V, E>(pre, a.pre, 0, a.D, col, width);
     const float inv_d = 1.f / (float)a.D;
+    const bool with_pre = a.pre && a.d_n;
     const long long worker = (long long)blockIdx.x * blockDim.y + threadIdx.y;
     for (long long row = worker; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
         float x[E], z[E], u[E], g[E], r[E], dn[E];
         load_row<T, V, E>(x, a.x, row * a.xs, a.D, col, width);
 #pragma unroll
-        for (int i = 0; i < E; ++i) { u[i] = x[i]; g[i] = 0.f; }
+        for (int i = 0; i < E; ++i) g[i] = 0.f;
         if (a.d_r) {
             if (a.dres) load_row<RT, V, E>(g, a.d_r, row * a.D, a.D, col, width);
             else load_row<T, V, E>(g, a.d_r, row * a.D, a.D, col, width);
         }
-        if (a.gate) {
-            load_row<T, V, E>(z, a.gate, row * a.gs, a.D, col, width);
-#pragma unroll
-            for (int i = 0; i < E; ++i) u[i] *= z[i] * sigmoid_hw(z[i]);
-        }
-        const bool with_pre = a.pre && a.d_n;
+        if (a.gate) load_row<T, V, E>(z, a.gate, row * a.gs, a.D, col, width);
         if (with_pre) {
             load_row<RT, V, E>(r, a.residual, row * a.rs, a.D, col, width);
             load_row<T, V, E>(dn, a.d_n, row * a.D, a.D, col, width);
         }
-        float e = 1.f;
-        if (a.post) {
-            float s[1] = {0.f};
+        const float e = a.post ? a.stats[2 * row] : 1.f, f = with_pre ? a.stats[2 * row + 1] : 0.f;
 #pragma unroll
-            for (int i = 0; i < E; ++i) s[0] = fmaf(u[i], u[i], s[0]);
-            sum(s);
-            e = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps));
-        }
+        for (int i = 0; i < E; ++i) u[i] = a.gate ? x[i] * (z[i] * sigmoid_hw(z[i])) : x[i];
+        float s[3] = {0.f, 0.f, 0.f};
         if (with_pre) {
-            float s[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                r[i] = fmaf(scale[i] * post[i], u[i] * e, r[i]);
-                s[0] = fmaf(r[i], r[i], s[0]);
-                s[1] = fmaf(dn[i] * pre[i], r[i], s[1]);
-            }
-            sum(s);
-            const float f = __builtin_amdgcn_rsqf(fmaf(s[0], inv_d, a.eps)), m = f * f * s[1] * inv_d;
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
+                const float w = scale[i] * post[i], wu = w * u[i];
+                r[i] = fmaf(e, wu, r[i]);
                 d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
-                g[i] = fmaf(f, fmaf(-r[i], m, dn[i] * pre[i]), g[i]);
+                dn[i] *= pre[i];
+                s[0] = fmaf(dn[i], r[i], s[0]);
+                g[i] = fmaf(f, dn[i], g[i]);
+                s[1] = fmaf(wu, g[i], s[1]);
+                s[2] = fmaf(wu, r[i], s[2]);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < E; ++i) s[1] = fmaf(scale[i] * post[i] * u[i], g[i], s[1]);
         }
-        if (a.dres) {
-            store_row<RT, V, E>(g, a.dres, row * a.D, a.D, col, width);
+        if (with_pre || a.post) sum(s);
+        const float m = f * f * f * s[0] * inv_d, mu = a.post ? e * e * (s[1] - m * s[2]) * inv_d : 0.f;
+        if (with_pre) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                d_scale[i] = fmaf(g[i], u[i] * e * post[i], d_scale[i]);
-                g[i] *= scale[i];
-            }
+            for (int i = 0; i < E; ++i) g[i] = fmaf(-r[i], m, g[i]);
         }
-        if (a.post) {
-            float q[1] = {0.f};
+        if (a.dres) store_row<RT, V, E>(g, a.dres, row * a.D, a.D, col, width);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                d_post[i] = fmaf(g[i], u[i] * e, d_post[i]);
-                g[i] *= post[i];
-                q[0] = fmaf(g[i], u[i], q[0]);
-            }
-            sum(q);
-            const float m = e * e * q[0] * inv_d;
-#pragma unroll
-            for (int i = 0; i < E; ++i) g[i] = e * fmaf(-u[i], m, g[i]);
+        for (int i = 0; i < E; ++i) {
+            const float ue = u[i] * e, dp = g[i] * scale[i];
+            d_scale[i] = fmaf(g[i], ue * post[i], d_scale[i]);
+            d_post[i] = fmaf(dp, ue, d_post[i]);
+            g[i] = e * fmaf(-u[i], mu, dp * post[i]);
         }
         if (a.gate) {
             float dz[E];
@@ -314,14 +304,14 @@ using namespace unetmi;
 extern "C" {
 
 int unetmi_block_norm_fwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
-                          const float* scale, const float* pre_weight, void* out, void* out_norm, void* stream) {
+                          const float* scale, const float* pre_weight, void* out, void* out_norm, float* stats, void* stream) {
     const int rc = norm_check(d, "block_norm_fwd");
     if (rc != UNETMI_OK) return rc;
     if (d->rows == 0) return UNETMI_OK;
     if (!x || !out || (pre_weight && !out_norm)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_fwd: null tensor pointer");
     if (!residual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_fwd: scale and pre_weight belong to a residual stream");
     NormArgs a = norm_args(*d, x, gate, post_weight, residual, scale, pre_weight);
-    a.out_r = out; a.out_n = out_norm;
+    a.out_r = out; a.out_n = out_norm; a.stats = stats;
     return norm_dispatch<false>(*d, a, norm_plan(*d, fwd_blocks(*d)), static_cast<hipStream_t>(stream));
 }
 
@@ -332,17 +322,17 @@ size_t unetmi_block_norm_bwd_workspace_bytes(const UnetmiNormDesc* d) {
 }
 
 int unetmi_block_norm_bwd(const UnetmiNormDesc* d, const void* x, const void* gate, const float* post_weight, const void* residual,
-                          const float* scale, const float* pre_weight, const void* d_out, const void* d_norm, void* dx, void* dgate,
+                          const float* scale, const float* pre_weight, const float* stats, const void* d_out, const void* d_norm, void* dx, void* dgate,
                           void* dresidual, float* dweights, void* ws, size_t ws_bytes, void* stream) {
     const int rc = norm_check(d, "block_norm_bwd");
     if (rc != UNETMI_OK) return rc;
     if (d->rows == 0) return api_fail(UNETMI_E_BAD_DESC, "block_norm_bwd: no rows");
-    if (!x || !dx || !dweights || !ws || (gate && !dgate) || (pre_weight && d_norm && !residual))
+    if (!x || !dx || !dweights || !ws || (gate && !dgate) || (pre_weight && d_norm && !residual) || ((post_weight || (pre_weight && d_norm)) && !stats))
         return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: null tensor pointer");
     if (!dresidual && (pre_weight || scale)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: scale and pre_weight belong to a residual stream");
     if (ws_bytes < unetmi_block_norm_bwd_workspace_bytes(d)) return api_fail(UNETMI_E_BAD_ARG, "block_norm_bwd: workspace too small");
     NormArgs a = norm_args(*d, x, gate, post_weight, residual, scale, pre_weight);
-    a.d_r = d_out; a.d_n = d_norm; a.dx = dx; a.dgate = dgate; a.dres = dresidual;
+    a.stats = const_cast<float*>(stats); a.d_r = d_out; a.d_n = d_norm; a.dx = dx; a.dgate = dgate; a.dres = dresidual;
     a.partial = static_cast<float*>(ws);
     const NormPlan p = norm_plan(*d, bwd_blocks(*d));
     hipStream_t s = static_cast<hipStream_t>(stream);

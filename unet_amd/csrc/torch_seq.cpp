@@ -317,28 +317,30 @@ struct NormIn {
     }
 };
 
-// (r, n) with a residual (n empty without pre_weight), else (p, empty)
-std::tuple<Tensor, Tensor> block_norm(const Tensor& x0, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
-                                      const Maybe& pre, double eps) {
+// (r, n) with a residual (n empty without pre_weight), else (p, empty); and the row statistics the backward call needs or empty
+std::tuple<Tensor, Tensor, Tensor> block_norm(const Tensor& x0, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
+                                              const Maybe& pre, double eps, bool want_stats) {
     TORCH_CHECK_VALUE(residual || (!scale && !pre), "unetmi::block_norm: scale and pre_weight belong to a residual stream");
     const NormIn in("block_norm", x0, gate, post, residual, scale, pre, eps, x0.scalar_type());
     const Tensor& x = in.x;
     const c10::DeviceGuard guard(x.device());
     const Tensor out = in.residual ? empty(x.sizes(), *in.residual) : empty(x.sizes(), x);
     const Tensor out_n = pre ? empty(x.sizes(), x) : empty({0}, x);
+    const Tensor stats = want_stats ? empty({x.size(0), 2}, x, at::kFloat) : empty({0}, x, at::kFloat);
     check(lib.norm_fwd(&in.d, ptr(x), ptr(in.gate), f32(post), ptr(in.residual), f32(scale), f32(pre), ptr(out), pre ? ptr(out_n) : nullptr,
-                       stream_of(x)), "unetmi_block_norm_fwd");
-    return {out, out_n};
+                       want_stats ? f32(stats) : nullptr, stream_of(x)), "unetmi_block_norm_fwd");
+    return {out, out_n, stats};
 }
 
 // (dx, dgate or empty, dresidual or empty, [dpost_weight, dscale, dpre_weight])
 std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_bwd(const Tensor& x0, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
-                                                          const Maybe& pre, double eps, const Maybe& d_out, const Maybe& d_norm, bool has_residual,
+                                                          const Maybe& pre, double eps, const Tensor& stats, const Maybe& d_out, const Maybe& d_norm, bool has_residual,
                                                           bool residual_f32) {
     const char* op = "block_norm_bwd";
     const at::ScalarType rtype = residual_f32 ? at::kFloat : x0.scalar_type();
     const NormIn in(op, x0, gate, post, residual, scale, pre, eps, rtype);
     const Tensor& x = in.x;
+    dense(stats, "stats", op, at::kFloat, x, {x.size(0), 2});
     dense(d_out, "d_out", op, has_residual ? rtype : x.scalar_type(), x, x.sizes());
     dense(d_norm, "d_norm", op, x.scalar_type(), x, x.sizes());
     const c10::DeviceGuard guard(x.device());
@@ -350,7 +352,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> block_norm_bwd(const Tensor& x0, cons
         return {dx, dgate, dres, dw};
     }
     const Tensor ws = scratch(lib.norm_bwd_bytes(&in.d), x);
-    check(lib.norm_bwd(&in.d, ptr(x), ptr(in.gate), f32(post), ptr(in.residual), f32(scale), f32(pre), ptr(d_out), ptr(d_norm), ptr(dx),
+    check(lib.norm_bwd(&in.d, ptr(x), ptr(in.gate), f32(post), ptr(in.residual), f32(scale), f32(pre), f32(stats), ptr(d_out), ptr(d_norm), ptr(dx),
                        gate ? ptr(dgate) : nullptr, has_residual ? ptr(dres) : nullptr, f32(dw), ptr(ws), ws.numel(), stream_of(x)),
           "unetmi_block_norm_bwd");
     return {dx, dgate, dres, dw};
@@ -500,8 +502,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
                                  const Maybe& scale, const Maybe& pre, double eps) {
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(block_norm)>("unetmi::block_norm");
-        auto [out, out_n] = op.call(x, gate, post, residual, scale, pre, eps);
-        ctx->save_for_backward({x, value(gate), value(post), value(scale), value(pre), pre ? *residual : Tensor()});
+        auto [out, out_n, stats] = op.call(x, gate, post, residual, scale, pre, eps, true);
+        ctx->save_for_backward({x, value(gate), value(post), value(scale), value(pre), pre ? *residual : Tensor(), stats});
         ctx->saved_data["eps"] = eps;
         ctx->saved_data["residual"] = residual.has_value();
         ctx->saved_data["f32"] = residual && residual->scalar_type() == at::kFloat;
@@ -518,7 +520,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
         const bool has = ctx->saved_data["residual"].toBool();
         static auto op = typed<decltype(block_norm_bwd)>("unetmi::block_norm_bwd");
         auto [dx, dgate, dres, dw] = op.call(s[0], maybe(s[1]), maybe(s[2]), maybe(s[5]), maybe(s[3]), maybe(s[4]), ctx->saved_data["eps"].toDouble(),
-                                             d_out, d_norm, has, ctx->saved_data["f32"].toBool());
+                                             s[6], d_out, d_norm, has, ctx->saved_data["f32"].toBool());
         Wanted wanted{ctx};
         out[0] = wanted.next(dx);
         out[1] = wanted.next(dgate, s[1].defined());
@@ -529,15 +531,15 @@ struct NormNode : torch::autograd::Function<NormNode> {
         return once("block_norm", std::move(out));
     }
 };
-std::tuple<Tensor, Tensor> block_norm_autograd(const Tensor& x, const Maybe& gate, const Maybe& post, const Maybe& residual, const Maybe& scale,
-                                               const Maybe& pre, double eps) {
+std::tuple<Tensor, Tensor, Tensor> block_norm_autograd(const Tensor& x, const Maybe& gate, const Maybe& post, const Maybe& residual,
+                                                       const Maybe& scale, const Maybe& pre, double eps, bool want_stats) {
     if (!recorded({&x}, {&gate, &post, &residual, &scale, &pre})) {
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(block_norm)>("unetmi::block_norm");
-        return op.call(x, gate, post, residual, scale, pre, eps);
+        return op.call(x, gate, post, residual, scale, pre, eps, want_stats);
     }
     const variable_list r = NormNode::apply(x, gate, post, residual, scale, pre, eps);
-    return {r[0], r[1]};
+    return {r[0], r[1], at::empty({0}, x.options().dtype(at::kFloat))};
 }
 
 }  // namespace
@@ -579,10 +581,10 @@ TORCH_LIBRARY_FRAGMENT(unetmi, m) {
           "Tensor marks, Tensor dy, Tensor? dstate_out, bool want_dstate) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
     m.def("ssm_scan_step(Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? z, Tensor? dt_bias, Tensor(a!) state, "
           "Tensor? slots, bool softplus) -> Tensor");
-    m.def("block_norm(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? residual, Tensor? scale, Tensor? pre_weight, float eps) "
-          "-> (Tensor, Tensor)");
+    m.def("block_norm(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? residual, Tensor? scale, Tensor? pre_weight, float eps, "
+          "bool want_stats) -> (Tensor, Tensor, Tensor)");
     m.def("block_norm_bwd(Tensor x, Tensor? gate, Tensor? post_weight, Tensor? residual, Tensor? scale, Tensor? pre_weight, float eps, "
-          "Tensor? d_out, Tensor? d_norm, bool has_residual, bool residual_f32) -> (Tensor, Tensor, Tensor, Tensor)");
+          "Tensor stats, Tensor? d_out, Tensor? d_norm, bool has_residual, bool residual_f32) -> (Tensor, Tensor, Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(unetmi, CUDA, m) {                                 // ROCm tensors dispatch here
     m.impl("seq_conv", seq_conv);

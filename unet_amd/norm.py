@@ -30,7 +30,7 @@ def block_norm(x, gate=None, post_weight=None, residual=None, scale=None, pre_we
         x, gate, residual = (None if t is None else t.reshape(-1, shape[-1]) for t in (x, gate, residual))
     if scale is not None and scale.numel() == 1:
         scale = scale.reshape(1).expand(shape[-1])
-    out, out_n = _ops.block_norm(x, gate, _packed(post_weight), residual, _packed(scale), _packed(pre_weight), eps)
+    out, out_n, _ = _ops.block_norm(x, gate, _packed(post_weight), residual, _packed(scale), _packed(pre_weight), eps, False)
     if not rows:
         out, out_n = out.view(shape), out_n if pre_weight is None else out_n.view(shape)
     return out if pre_weight is None else (out, out_n)

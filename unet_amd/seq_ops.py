@@ -72,13 +72,14 @@ def _(x, dt, A, B, C, D, z, dt_bias, state, slots, softplus):
 
 
 @torch.library.register_fake("unetmi::block_norm")
-def _(x, gate, post_weight, residual, scale, pre_weight, eps):
+def _(x, gate, post_weight, residual, scale, pre_weight, eps, want_stats):
     return (x.new_empty(x.shape, dtype=x.dtype if residual is None else residual.dtype),
-            x.new_empty((0,) if pre_weight is None else x.shape))
+            x.new_empty((0,) if pre_weight is None else x.shape),
+            x.new_empty((x.shape[0], 2) if want_stats else (0,), dtype=torch.float32))
 
 
 @torch.library.register_fake("unetmi::block_norm_bwd")
-def _(x, gate, post_weight, residual, scale, pre_weight, eps, d_out, d_norm, has_residual, residual_f32):
+def _(x, gate, post_weight, residual, scale, pre_weight, eps, stats, d_out, d_norm, has_residual, residual_f32):
     return (x.new_empty(x.shape), x.new_empty((0,) if gate is None else x.shape),
             x.new_empty(x.shape if has_residual else (0,), dtype=torch.float32 if residual_f32 else x.dtype),
             x.new_empty((3, x.shape[1]), dtype=torch.float32))
