@@ -397,6 +397,13 @@ def test_block_norm(device, rows, D, gate, post, residual, scale, pre, xt, rt):
             held(g, want["d_" + short], room["d_" + short], 192 + (rows if g.dim() == 1 else 0), "d " + k)
 
 
+@pytest.mark.parametrize("xt,rt", [(F32, F32), (BF16, BF16), (BF16, F32)])
+@pytest.mark.parametrize("rows,D", [(20000, 40), (9000, 520), (2000, 1100), (600, 5001), (520, 8192)])
+def test_block_norm_of_many_rows(device, rows, D, xt, rt):
+    """More rows than blocks: a block's threads go on to the next row, over one wave and over up to sixteen."""
+    test_block_norm(device, rows, D, 1, 1, 1, 1, 1, xt, rt)
+
+
 def test_block_norm_without_some_gradients_and_with_a_single_scale(device):
     """Only one of the two outputs used; the scale as one value (its gradient the sum over the channels)."""
     from unet_amd import norm

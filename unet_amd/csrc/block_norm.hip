@@ -4,14 +4,18 @@
 //     r = residual + scale p           the stream                      (the output p if there is no residual)
 //     n = w_pre r / rms(r)             the norm before the next block
 // Rows are read once and written once (three inputs, two outputs: ten bytes a bfloat16 element, about 16 operations), so
-// HBM bounds both directions.  A thread holds E elements of a row in fp32: eight, rows of up to 512 elements one wave and
-// wider ones a block of up to eight waves; sixteen beyond 4096 elements.  Blocks walk over rows: the weights stay in registers, and in the
-// backward kernel so do their gradients' partial sums, added up in a fixed order by a second kernel.  Measured: forward
-// 16387 x 2048 bf16 61 us (5.5 TB/s), 16032 x 1285 fp32 81 us (5.1 TB/s), its backward 132 us (5.0 TB/s) and 6 for the sums;
-// 64 rows of 2048 in 4 us.
+// HBM bounds both directions.  A thread holds eight elements of a row in fp32: rows of up to 512 elements are one wave, wider
+// ones a block of up to sixteen.  Blocks walk over rows.  Forward, the weights stay in registers; backward in LDS (a wave a SIMD
+// more, and rows of 8192 without spills: 4096 x 8192 bf16 299 -> 114 us), the weights' gradients as partial sums in registers,
+// added up in a fixed order by a second kernel.  Measured: forward 16387 x 2048 bf16 61 us (5.5 TB/s), 16032 x 1285 fp32 80 us
+// (5.1 TB/s), backward 110 us (4.9 TB/s) and 139 us (4.7 TB/s) and 5 for the sums; 64 rows of 2048 in 4 us.
 #include "seq_common.hpp"
 
+#include <type_traits>
+
 namespace unetmi {
+
+constexpr int kElems = 8;                // of a row, per thread
 
 struct NormArgs {
     const void *x, *gate;                 // gate may be null
@@ -29,41 +33,52 @@ struct NormArgs {
     float* partial;                       // [workers, 3, D]: post, scale, pre
 };
 
-__device__ __forceinline__ float wave_sum(float v) {
+__device__ __forceinline__ float row_sum16(float v) {                 // over the lane's row of 16
     v += dpp<0xB1>(v);
     v += dpp<0x4E>(v);
     v += dpp<0x124>(v);
-    v += dpp<0x128>(v);
+    return v + dpp<0x128>(v);
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v = row_sum16(v);
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
 
+// threadIdx.y, which is the same for a wave: a block has one row, or a row per wave
+__device__ __forceinline__ int wave_row() { return __builtin_amdgcn_readfirstlane(threadIdx.y); }
+
 // Sums over a row's threads.  One wave: no LDS.  More: the two halves of `red` are used in turn, so that one barrier per
 // call is enough.
 struct RowSum {
-    float* red;                           // [2][8][3]
+    float* red;                           // [2][16][3]
     int waves, wave, turn = 0;
     template <int M>
     __device__ __forceinline__ void operator()(float (&v)[M]) {
 #pragma unroll
         for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
         if (waves == 1) return;
-        float* mine = red + turn * 24;
+        float* mine = red + turn * 48;
         turn ^= 1;
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int m = 0; m < M; ++m) mine[wave * 3 + m] = v[m];
         __syncthreads();
+        const int w = threadIdx.x & 15;                               // every sixteen lanes add up the waves' sums
 #pragma unroll
-        for (int m = 0; m < M; ++m) {
-            float s = 0.f;
-            for (int w = 0; w < waves; ++w) s += mine[w * 3 + m];
-            v[m] = s;
-        }
+        for (int m = 0; m < M; ++m) v[m] = w < waves ? mine[w * 3 + m] : 0.f;
+#pragma unroll
+        for (int m = 0; m < M; ++m) v[m] = row_sum16(v[m]);
     }
 };
 
-// a thread's elements of a row: E / V vectors, `width` threads apart
+// a thread's elements of a row: E / V vectors, `width` threads apart.  The row's start is the same for a wave (scalar registers)
+// and a thread's place in it an offset of 32 bits: a dozen 64-bit addresses a thread would cost the backward kernel a wave a SIMD.
+template <class T>
+__device__ __forceinline__ T* within(T* row, int c) {
+    typedef std::conditional_t<std::is_const_v<T>, const char, char> byte;
+    return reinterpret_cast<T*>(reinterpret_cast<byte*>(row) + (unsigned)c * (unsigned)sizeof(T));
+}
 template <class T, int V, int E>
 __device__ __forceinline__ void load_row(float (&o)[E], const void* p, long long row, int D, int col, int width) {
 #pragma unroll
@@ -71,7 +86,7 @@ __device__ __forceinline__ void load_row(float (&o)[E], const void* p, long long
         const int c = (j * width + col) * V;
         Pack<T, V> k;
         k.zero();
-        if (c < D) k.load_n(static_cast<const T*>(p) + row + c, D - c);
+        if (c < D) k.load_n(within(static_cast<const T*>(p) + row, c), D - c);
 #pragma unroll
         for (int v = 0; v < V; ++v) o[j * V + v] = k.get(v);
     }
@@ -84,14 +99,14 @@ __device__ __forceinline__ void store_row(const float (&o)[E], void* p, long lon
         Pack<T, V> k;
 #pragma unroll
         for (int v = 0; v < V; ++v) k.set(v, o[j * V + v]);
-        if (c < D) k.store_n(static_cast<T*>(p) + row + c, D - c);
+        if (c < D) k.store_n(within(static_cast<T*>(p) + row, c), D - c);
     }
 }
 
-template <class T, class RT, int E>
-__global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
-    constexpr int V = kVector<T>;
-    __shared__ float red[48];
+template <class T, class RT>
+__global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
+    constexpr int V = kVector<T>, E = kElems;
+    __shared__ float red[96];
     const int width = blockDim.x, col = threadIdx.x;
     RowSum sum{red, width >> 6, col >> 6};
     float post[E], scale[E], pre[E];
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
     if (a.scale) load_row<float, V, E>(scale, a.scale, 0, a.D, col, width);
     if (a.pre) load_row<float, V, E>(pre, a.pre, 0, a.D, col, width);
     const float inv_d = 1.f / (float)a.D;
-    for (long long row = (long long)blockIdx.x * blockDim.y + threadIdx.y; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
+    for (long long row = (long long)blockIdx.x * blockDim.y + wave_row(); row < a.rows; row += (long long)gridDim.x * blockDim.y) {
         float u[E], r[E];
         load_row<T, V, E>(u, a.x, row * a.xs, a.D, col, width);
         if (a.residual) load_row<RT, V, E>(r, a.residual, row * a.rs, a.D, col, width);
@@ -149,23 +164,35 @@ __global__ __launch_bounds__(512) void block_norm_fwd_kernel(NormArgs a) {
 // so the three sums are taken together and a row waits once (16032 x 1285 fp32: 175 us with e, f and the means one after the
 // other).  r is computed again from the residual, which has to be read anyway: a stream stored in 16 bits would leave its
 // rounding in the weights' gradients (2e-3 of dscale and dw_pre over a few rows).
-template <class T, class RT, int E>
-__global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
-    constexpr int V = kVector<T>;
-    __shared__ float red[48];
+template <class T, class RT, int THREADS>
+__global__ __launch_bounds__(THREADS) void block_norm_bwd_kernel(NormArgs a) {
+    constexpr int V = kVector<T>, E = kElems;
+    __shared__ float red[96];
+    extern __shared__ f32x4 own[];        // [post, scale, pre][half][thread of a row]
     const int width = blockDim.x, col = threadIdx.x;
     RowSum sum{red, width >> 6, col >> 6};
-    float post[E], scale[E], pre[E], d_post[E], d_scale[E], d_pre[E];
+    float d_post[E], d_scale[E], d_pre[E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) { post[i] = scale[i] = 1.f; pre[i] = 0.f; d_post[i] = d_scale[i] = d_pre[i] = 0.f; }
-    if (a.post) load_row<float, V, E>(post, a.post, 0, a.D, col, width);
-    if (a.scale) load_row<float, V, E>(scale, a.scale, 0, a.D, col, width);
-    if (a.pre) load_row<float, V, E>(pre, a.pre, 0, a.D, col, width);
+    for (int i = 0; i < E; ++i) d_post[i] = d_scale[i] = d_pre[i] = 0.f;
+    if (threadIdx.y == 0) {
+        const float* const w[3] = {a.post, a.scale, a.pre};
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            float v[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[i] = 1.f;
+            if (w[k]) load_row<float, V, E>(v, w[k], 0, a.D, col, width);
+            own[2 * k * width + col] = f32x4{v[0], v[1], v[2], v[3]};
+            own[(2 * k + 1) * width + col] = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    }
+    __syncthreads();
+    auto weight = [&](int k, int half) { return own[(2 * k + half) * width + col]; };
     const float inv_d = 1.f / (float)a.D;
     const bool with_pre = a.pre && a.d_n;
-    const long long worker = (long long)blockIdx.x * blockDim.y + threadIdx.y;
+    const long long worker = (long long)blockIdx.x * blockDim.y + wave_row();
     for (long long row = worker; row < a.rows; row += (long long)gridDim.x * blockDim.y) {
-        float x[E], z[E], u[E], g[E], r[E], dn[E];
+        float x[E], z[E], g[E], r[E], dn[E];
         load_row<T, V, E>(x, a.x, row * a.xs, a.D, col, width);
 #pragma unroll
         for (int i = 0; i < E; ++i) g[i] = 0.f;
@@ -179,24 +206,31 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
             load_row<T, V, E>(dn, a.d_n, row * a.D, a.D, col, width);
         }
         const float e = a.post ? a.stats[2 * row] : 1.f, f = with_pre ? a.stats[2 * row + 1] : 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) u[i] = a.gate ? x[i] * (z[i] * sigmoid_hw(z[i])) : x[i];
         float s[3] = {0.f, 0.f, 0.f};
-        if (with_pre) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float w = scale[i] * post[i], wu = w * u[i];
-                r[i] = fmaf(e, wu, r[i]);
-                d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
-                dn[i] *= pre[i];
-                s[0] = fmaf(dn[i], r[i], s[0]);
-                g[i] = fmaf(f, dn[i], g[i]);
-                s[1] = fmaf(wu, g[i], s[1]);
-                s[2] = fmaf(wu, r[i], s[2]);
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 w = weight(0, h) * weight(1, h), pre = weight(2, h);
+            float wu[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) wu[k] = w[k] * x[4 * h + k];
+            if (a.gate) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) wu[k] *= z[4 * h + k] * sigmoid_hw(z[4 * h + k]);
             }
-        } else {
+            if (with_pre) {
 #pragma unroll
-            for (int i = 0; i < E; ++i) s[1] = fmaf(scale[i] * post[i] * u[i], g[i], s[1]);
+                for (int k = 0; k < 4; ++k) {
+                    const int i = 4 * h + k;
+                    r[i] = fmaf(e, wu[k], r[i]);
+                    d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
+                    const float dp = dn[i] * pre[k];
+                    s[0] = fmaf(dp, r[i], s[0]);
+                    g[i] = fmaf(f, dp, g[i]);
+                    s[2] = fmaf(wu[k], r[i], s[2]);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[1] = fmaf(wu[k], g[4 * h + k], s[1]);
         }
         if (with_pre || a.post) sum(s);
         const float m = f * f * f * s[0] * inv_d, mu = a.post ? e * e * (s[1] - m * s[2]) * inv_d : 0.f;
@@ -206,22 +240,21 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
         }
         if (a.dres) store_row<RT, V, E>(g, a.dres, row * a.D, a.D, col, width);
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float ue = u[i] * e, dp = g[i] * scale[i];
-            d_scale[i] = fmaf(g[i], ue * post[i], d_scale[i]);
-            d_post[i] = fmaf(dp, ue, d_post[i]);
-            g[i] = e * fmaf(-u[i], mu, dp * post[i]);
-        }
-        if (a.gate) {
-            float dz[E];
+        for (int h = 0; h < 2; ++h) {
+            const f32x4 post = weight(0, h), scale = weight(1, h);
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const float sg = sigmoid_hw(z[i]);
-                dz[i] = g[i] * x[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
-                g[i] *= z[i] * sg;
+            for (int k = 0; k < 4; ++k) {
+                const int i = 4 * h + k;
+                const float sg = a.gate ? sigmoid_hw(z[i]) : 1.f, silu = a.gate ? z[i] * sg : 1.f;
+                const float u = x[i] * silu, ue = u * e, dp = g[i] * scale[k];
+                d_scale[i] = fmaf(g[i], ue * post[k], d_scale[i]);
+                d_post[i] = fmaf(dp, ue, d_post[i]);
+                const float du = e * fmaf(-u, mu, dp * post[k]);
+                g[i] = du * silu;
+                if (a.gate) z[i] = du * x[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
             }
-            store_row<T, V, E>(dz, a.dgate, row * a.D, a.D, col, width);
         }
+        if (a.gate) store_row<T, V, E>(z, a.dgate, row * a.D, a.D, col, width);
         store_row<T, V, E>(g, a.dx, row * a.D, a.D, col, width);
     }
     float* out = a.partial + worker * 3 * a.D;
@@ -232,10 +265,6 @@ __global__ __launch_bounds__(512) void block_norm_bwd_kernel(NormArgs a) {
 
 namespace {
 
-// Elements a thread: sixteen where eight would need more than eight waves a row -- blocks of sixteen waves leave the backward
-// kernel 128 registers, which spilled (16032 x 1285 fp32 bounded for them: 286 us against 150).
-int norm_elems(const UnetmiNormDesc& d) { return d.channels <= 4096 ? 8 : 16; }
-
 struct NormPlan {
     int width, per_block;                 // threads per row, rows per block
     unsigned blocks;
@@ -243,8 +272,7 @@ struct NormPlan {
 
 NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
     NormPlan p;
-    const int e = norm_elems(d);
-    p.width = ((d.channels + e - 1) / e + 63) / 64 * 64;
+    p.width = ((d.channels + kElems - 1) / kElems + 63) / 64 * 64;
     p.per_block = p.width == 64 ? 4 : 1;
     long long n = (d.rows + p.per_block - 1) / p.per_block;
     p.blocks = (unsigned)(n < 1 ? 1 : (n > most_blocks ? most_blocks : n));
@@ -252,10 +280,16 @@ NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
 }
 
 // Waves per CU: forward 64, about three times what is resident, so that CUs that end early find work (16387 x 2048 bf16: 61 us,
-// 67 with 32 and 65 with 16; 16032 x 1285 fp32: 81, 78 and 85).  Backward 12, what is resident, since every block more costs
-// 12 bytes a column of partial sums (16032 x 1285 fp32: 132 us and 6 for the sums; 8 waves 153, 16 waves 173, 24 141 and 12).
+// 67 with 32 and 65 with 16; 16032 x 1285 fp32: 81, 78 and 85).
 long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 64 / (p.width * p.per_block / 64); }
-long long bwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 12 / (p.width * p.per_block / 64); }
+// Backward: whole blocks a CU, all resident (every block more costs 12 bytes a column of partial sums, and 1.2 blocks a CU take
+// as long as two), sixteen waves of them with 16-bit activations and eight with fp32, whose rows are twice the bytes: 16387 x 2048
+// bf16 145, 119 and 110 us with 8, 12 and 16 waves, 16032 x 1285 bf16 194, 127 and 115, fp32 139, 151 and 156.
+long long bwd_blocks(const UnetmiNormDesc& d) {
+    const NormPlan p = norm_plan(d, 1);
+    const int per_cu = (d.dtype == UNETMI_DTYPE_BF16 ? 16 : 8) / (p.width * p.per_block / 64);
+    return 256 * (per_cu ? per_cu : 1);
+}
 
 int norm_check(const UnetmiNormDesc* d, const char* what) {
     const std::string w = what;
@@ -270,21 +304,20 @@ int norm_check(const UnetmiNormDesc* d, const char* what) {
     return UNETMI_OK;
 }
 
-template <class T, class RT, int E, bool BWD>
+template <class T, class RT, bool BWD>
 int norm_launch(const NormArgs& a, const NormPlan& p, hipStream_t s) {
     const dim3 block(p.width, p.per_block);
-    if (BWD) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, E>), dim3(p.blocks), block, 0, s, a);
-    else hipLaunchKernelGGL((block_norm_fwd_kernel<T, RT, E>), dim3(p.blocks), block, 0, s, a);
+    const size_t lds = 6 * sizeof(f32x4) * p.width;
+    if (BWD && p.width <= 512) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, 512>), dim3(p.blocks), block, lds, s, a);
+    else if (BWD) hipLaunchKernelGGL((block_norm_bwd_kernel<T, RT, 1024>), dim3(p.blocks), block, lds, s, a);
+    else hipLaunchKernelGGL((block_norm_fwd_kernel<T, RT>), dim3(p.blocks), block, 0, s, a);
     return launched(BWD ? "block_norm_bwd" : "block_norm_fwd");
 }
 
 template <bool BWD>
 int norm_dispatch(const UnetmiNormDesc& d, const NormArgs& a, const NormPlan& p, hipStream_t s) {
-    const bool wide = norm_elems(d) == 16;
-    if (d.dtype == UNETMI_DTYPE_F32) return wide ? norm_launch<float, float, 16, BWD>(a, p, s) : norm_launch<float, float, 8, BWD>(a, p, s);
-    if (d.residual_dtype == UNETMI_DTYPE_F32)
-        return wide ? norm_launch<__bf16, float, 16, BWD>(a, p, s) : norm_launch<__bf16, float, 8, BWD>(a, p, s);
-    return wide ? norm_launch<__bf16, __bf16, 16, BWD>(a, p, s) : norm_launch<__bf16, __bf16, 8, BWD>(a, p, s);
+    if (d.dtype == UNETMI_DTYPE_F32) return norm_launch<float, float, BWD>(a, p, s);
+    return d.residual_dtype == UNETMI_DTYPE_F32 ? norm_launch<__bf16, float, BWD>(a, p, s) : norm_launch<__bf16, __bf16, BWD>(a, p, s);
 }
 
 NormArgs norm_args(const UnetmiNormDesc& d, const void* x, const void* gate, const float* post, const void* residual, const float* scale,
