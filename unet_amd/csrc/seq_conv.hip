@@ -2,13 +2,16 @@
 //     y_t = act(bias + sum_k w_k x_{t-K+1+k}),   K = 2..4, act = SiLU or none,
 // over the K-1 inputs before the first one (a state, or zeros), its gradients and its form for single tokens.
 // Two or three operations per tap against one read and one write of HBM: the traffic bounds all three kernels.  A thread
-// keeps one vector of channels (16 bytes) and walks along time with the last
-// K-1 inputs in registers, so a row is read once per time segment plus K-1 rows that the caches still hold.  Measured:
-// forward 32 x 501 x 768 fp32 20 us (4.9 TB/s), 8 x 4096 x 2048 bf16 of lengths 0..4096 43 us; backward of the former 36 us
-// (4.1 TB/s) and 4 for the sums; 256 tokens x 2048 channels bf16 5 us.
+// keeps four channels and walks along time with the last K-1 inputs in registers, so a row is read once per time segment plus
+// K-1 rows that the caches still hold.  Four also of 16 bits, 512 bytes a wave and row: eight take so many registers that two
+// waves a SIMD remain of four (8 x 4096 x 2048 bf16 forward 54 -> 47 us, backward 113 -> 98; 32 x 501 x 768 13.8 -> 11.1 and 31
+// -> 27).  Measured: forward 32 x 501 x 768 fp32 20 us (4.9 TB/s), 8 x 4096 x 2048 bf16 of lengths 0..4096 41 us; backward of
+// the former 36 us (4.1 TB/s) and 4 for the sums; 256 tokens x 2048 channels bf16 4 us.
 #include "seq_common.hpp"
 
 namespace unetmi {
+
+constexpr int kConvV = 4;               // channels per thread
 
 struct ConvSeqArgs {
     const void* x;
@@ -360,7 +363,7 @@ int launch_sum_rows(const float* rows, int R, SumPiece a, SumPiece b, SumPiece c
 namespace {
 
 struct ConvSeqPlan {
-    int V, cw_log2, steps, nblk_t, nblk_c;
+    int cw_log2, steps, nblk_t, nblk_c;
 };
 
 // threads along the channels: as many (a power of two, at most a wave) as there are channel vectors; the rest of the
@@ -369,8 +372,7 @@ struct ConvSeqPlan {
 // blocks, 41 with 8; forward of 8 x 4096 x 2048 bf16: 43.5 us with 32 rows, 45.6 with 16).
 ConvSeqPlan conv_plan(const UnetmiSeqConvDesc& d) {
     ConvSeqPlan p;
-    p.V = d.dtype == UNETMI_DTYPE_BF16 ? 8 : 4;
-    const int nv = (d.channels + p.V - 1) / p.V;
+    const int nv = (d.channels + kConvV - 1) / kConvV;
     p.cw_log2 = 0;
     while ((1 << p.cw_log2) < nv && p.cw_log2 < 6) ++p.cw_log2;
     p.nblk_c = (nv + (1 << p.cw_log2) - 1) >> p.cw_log2;
@@ -415,7 +417,7 @@ int conv_taps(const UnetmiSeqConvDesc& d, A&&... args) {
 }
 template <template <class, int, int, bool> class F, class... A>
 int conv_dispatch(const UnetmiSeqConvDesc& d, A&&... args) {
-    return d.dtype == UNETMI_DTYPE_BF16 ? conv_taps<F, __bf16, kVector<__bf16>>(d, args...) : conv_taps<F, float, kVector<float>>(d, args...);
+    return d.dtype == UNETMI_DTYPE_BF16 ? conv_taps<F, __bf16, kConvV>(d, args...) : conv_taps<F, float, kConvV>(d, args...);
 }
 
 template <class T, int V, int K, bool ACT>
@@ -461,8 +463,6 @@ struct RunStep {
         return launched("seq_conv_step");
     }
 };
-
-
 
 }  // namespace
 }  // namespace unetmi
