@@ -50,6 +50,8 @@ struct Pack<T, 1> {
     T v;
     __device__ __forceinline__ void load(const T* p) { v = *p; }
     __device__ __forceinline__ void store(T* p) const { *p = v; }
+    __device__ __forceinline__ void load_n(const T* p, int n) { v = n > 0 ? *p : (T)0.f; }
+    __device__ __forceinline__ void store_n(T* p, int n) const { if (n > 0) *p = v; }
     __device__ __forceinline__ float get(int) const { return widen(v); }
     __device__ __forceinline__ void set(int, float f) { v = (T)f; }
     __device__ __forceinline__ void zero() { v = (T)0.f; }
