@@ -397,6 +397,21 @@ def test_block_norm(device, rows, D, gate, post, residual, scale, pre, xt, rt):
             held(g, want["d_" + short], room["d_" + short], 192 + (rows if g.dim() == 1 else 0), "d " + k)
 
 
+@pytest.mark.parametrize("size,eps", [(1e14, 1e-6), (1e-14, 0.0)])
+def test_block_norm_of_large_and_small_values(device, size, eps):
+    """Rows whose squares are far from 1: every part scales with them or does not."""
+    from unet_amd import norm
+    names = ("x", "gate", "post_weight", "residual", "scale", "pre_weight")
+    t = [rnd((6, 200), 1) * size, rnd((6, 200), 2), rnd((200,), 3) * size, rnd((6, 200), 4) * size, rnd((200,), 5), rnd((200,), 6)]
+    d_out, d_n = rnd((6, 200), 7) / size, rnd((6, 200), 8)
+    leaves = {k: v.to(device).requires_grad_() for k, v in zip(names, t)}
+    grads = torch.autograd.grad(norm.block_norm(**leaves, eps=eps), list(leaves.values()), (d_out.to(device), d_n.to(device)))
+    want, room = (norm64(*t, eps, d_out, d_n, magnitude=m) for m in (False, True))
+    for k, g in zip(leaves, grads):
+        short = k.replace("_weight", "")
+        held(g, want["d_" + short], room["d_" + short], 192 + (6 if g.dim() == 1 else 0), "d " + k)
+
+
 @pytest.mark.parametrize("xt,rt", [(F32, F32), (BF16, BF16), (BF16, F32)])
 @pytest.mark.parametrize("rows,D", [(20000, 40), (9000, 520), (2000, 1100), (600, 5001), (520, 8192)])
 def test_block_norm_of_many_rows(device, rows, D, xt, rt):

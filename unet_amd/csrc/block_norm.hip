@@ -160,7 +160,8 @@ __global__ __launch_bounds__(1024) void block_norm_fwd_kernel(NormArgs a) {
 //     dresidual = dr,  dscale = sum dr p,  dp = scale dr            (without a residual dp = d_r)
 //     du = e (q - u e^2 mean(q u)),  q = dp w_post                  dw_post = sum dp u e
 //     dx = du silu(gate),  dgate = du x silu'(gate)
-// With w = scale w_post the second mean is linear in the first one, sum(q u) = sum(w u (d_r + f g)) - f^3 mean(g r) sum(w u r),
+// With the rows in units of their rms, v = u e and n = r f, and w = scale w_post, the second mean is linear in the first one,
+//     m = f mean(g n),  dr = d_r + f g - m n,  sum(q v) = sum(w v (d_r + f g)) - m sum(w v n),
 // so the three sums are taken together and a row waits once (16032 x 1285 fp32: 175 us with e, f and the means one after the
 // other).  r is computed again from the residual, which has to be read anyway: a stream stored in 16 bits would leave its
 // rounding in the weights' gradients (2e-3 of dscale and dw_pre over a few rows).
@@ -210,30 +211,30 @@ __global__ __launch_bounds__(THREADS) void block_norm_bwd_kernel(NormArgs a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const f32x4 w = weight(0, h) * weight(1, h), pre = weight(2, h);
-            float wu[4];
+            float wv[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) wu[k] = w[k] * x[4 * h + k];
+            for (int k = 0; k < 4; ++k) wv[k] = w[k] * (x[4 * h + k] * e);
             if (a.gate) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) wu[k] *= z[4 * h + k] * sigmoid_hw(z[4 * h + k]);
+                for (int k = 0; k < 4; ++k) wv[k] *= z[4 * h + k] * sigmoid_hw(z[4 * h + k]);
             }
             if (with_pre) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int i = 4 * h + k;
-                    r[i] = fmaf(e, wu[k], r[i]);
-                    d_pre[i] = fmaf(dn[i], r[i] * f, d_pre[i]);
+                    r[i] = (r[i] + wv[k]) * f;
+                    d_pre[i] = fmaf(dn[i], r[i], d_pre[i]);
                     const float dp = dn[i] * pre[k];
                     s[0] = fmaf(dp, r[i], s[0]);
                     g[i] = fmaf(f, dp, g[i]);
-                    s[2] = fmaf(wu[k], r[i], s[2]);
+                    s[2] = fmaf(wv[k], r[i], s[2]);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[1] = fmaf(wu[k], g[4 * h + k], s[1]);
+            for (int k = 0; k < 4; ++k) s[1] = fmaf(wv[k], g[4 * h + k], s[1]);
         }
         if (with_pre || a.post) sum(s);
-        const float m = f * f * f * s[0] * inv_d, mu = a.post ? e * e * (s[1] - m * s[2]) * inv_d : 0.f;
+        const float m = f * (s[0] * inv_d), mv = a.post ? (s[1] - m * s[2]) * inv_d : 0.f;
         if (with_pre) {
 #pragma unroll
             for (int i = 0; i < E; ++i) g[i] = fmaf(-r[i], m, g[i]);
@@ -246,10 +247,10 @@ __global__ __launch_bounds__(THREADS) void block_norm_bwd_kernel(NormArgs a) {
             for (int k = 0; k < 4; ++k) {
                 const int i = 4 * h + k;
                 const float sg = a.gate ? sigmoid_hw(z[i]) : 1.f, silu = a.gate ? z[i] * sg : 1.f;
-                const float u = x[i] * silu, ue = u * e, dp = g[i] * scale[k];
-                d_scale[i] = fmaf(g[i], ue * post[k], d_scale[i]);
-                d_post[i] = fmaf(dp, ue, d_post[i]);
-                const float du = e * fmaf(-u, mu, dp * post[k]);
+                const float v = x[i] * e * silu, dp = g[i] * scale[k];
+                d_scale[i] = fmaf(g[i], v * post[k], d_scale[i]);
+                d_post[i] = fmaf(dp, v, d_post[i]);
+                const float du = e * fmaf(-v, mv, dp * post[k]);
                 g[i] = du * silu;
                 if (a.gate) z[i] = du * x[i] * sg * fmaf(z[i], 1.f - sg, 1.f);
             }
