@@ -622,6 +622,30 @@ def test_a_captured_backward_beside_an_eager_graph(device):
             assert torch.equal(got, want), name
 
 
+def test_a_captured_backward_past_an_eager_input(device):
+    """An input that an eager graph made does not stand in the way where its gradient is not asked for."""
+    from unet_amd import ssm
+    base = rnd((2, 40, 64), 1).to(device).requires_grad_()
+    x = base * 2
+    w = rnd((64, 4), 2).to(device).requires_grad_()
+    dy = rnd((2, 40, 64), 3).to(device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(ssm.causal_conv(x, w), w, dy)
+    with pytest.raises(RuntimeError, match="eager graph on the default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(ssm.causal_conv(x, w), x, dy)
+    want, = torch.autograd.grad(ssm.causal_conv(x, w.detach().requires_grad_()), x, dy)
+    assert torch.isfinite(want).all()
+    leaf = w.detach().requires_grad_()
+    want, = torch.autograd.grad(ssm.causal_conv(x, leaf), leaf, dy)
+    for _ in range(3):
+        got.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
 def test_tokens_in_a_graph(device):
     """A block's token step captured once and replayed over a growing stream, two graphs in turn on two caches, with eager
     work between: every token is the eager one, bit for bit."""

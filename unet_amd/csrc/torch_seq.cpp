@@ -389,8 +389,9 @@ void joins_capture(const char* what) {
     if (here.id() == 0) return;                                       // the default stream is never captured
     const auto node = torch::autograd::get_current_node();
     if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-    for (const auto& edge : node->next_edges()) {
-        const auto stream = edge.function ? edge.function->stream() : std::nullopt;
+    for (size_t i = 0; i < node->num_outputs(); ++i) {
+        const auto& to = node->next_edge(i).function;
+        const auto stream = to && node->task_should_compute_output(i) ? to->stream() : std::nullopt;
         TORCH_CHECK(!stream || stream->id() != 0, "unet_amd: the backward pass of ", what, " is being captured into a graph, but an input's gradient "
                     "belongs to an eager graph on the default stream: free that graph (its outputs) before the capture, or run it on another stream");
     }
