@@ -384,7 +384,8 @@ variable_list once(const char* what, variable_list gradients) {
 // A captured backward pass cannot hand its gradients to a node that lives on the default stream, as the leaves' nodes do
 // while an eager graph of the same leaves is alive: waiting on that stream breaks the capture, and ends the process later.
 // Said here, before that wait.
-void joins_capture(const char* what) {
+void joins_capture(const char* what, const Tensor& x) {
+    if (!x.is_cuda()) return;                                         // no stream (kernels that stand in on the CPU)
     const auto here = c10::hip::getCurrentHIPStream();
     if (here.id() == 0) return;                                       // the default stream is never captured
     const auto node = torch::autograd::get_current_node();
@@ -412,6 +413,35 @@ auto typed(const char* name) {
     return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 
+// Forward-mode derivatives are not built.  A tensor that carries a tangent need not require a gradient, so every op asks by
+// itself, before the kernel would drop the tangent without a word.
+template <class T>
+void no_tangent(const char*, const T&) {}
+void no_tangent(const char* what, const Tensor& t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), "unet_amd: ", what, " has no forward-mode derivative");
+}
+void no_tangent(const char* what, const Maybe& t) {
+    if (t) no_tangent(what, *t);
+}
+template <class... A>
+void no_tangents(const char* what, const A&... args) {
+    (no_tangent(what, args), ...);
+}
+// the _bwd and _step ops below the autograd key: they record nothing
+template <const auto& Name, auto Kernel>
+struct Below;
+template <const auto& Name, class R, class... A, R (*Kernel)(A...)>
+struct Below<Name, Kernel> {
+    static R call(A... args) {
+        no_tangents(Name, args...);
+        at::AutoDispatchBelowADInplaceOrView below;
+        static auto op = typed<R(A...)>(Name);
+        return op.call(args...);
+    }
+};
+constexpr char kConvBwd[] = "unetmi::seq_conv_bwd", kScanBwd[] = "unetmi::ssm_scan_bwd", kNormBwd[] = "unetmi::block_norm_bwd",
+               kConvStep[] = "unetmi::seq_conv_step", kScanStep[] = "unetmi::ssm_scan_step";
+
 struct ConvNode : torch::autograd::Function<ConvNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& state,
                                  const Maybe& lengths, bool silu, bool want_state) {
@@ -426,8 +456,8 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(7);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        joins_capture("causal_conv");
         const variable_list s = ctx->get_saved_variables();
+        joins_capture("causal_conv", s[0]);
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
         const Maybe dout = grads[1].defined() && grads[1].dim() == 3 ? Maybe(grads[1].contiguous()) : Maybe();
         static auto op = typed<decltype(seq_conv_bwd)>("unetmi::seq_conv_bwd");
@@ -442,6 +472,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
 };
 std::tuple<Tensor, Tensor> seq_conv_autograd(const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& state, const Maybe& lengths,
                                              bool silu, bool want_state) {
+    no_tangents("causal_conv", x, weight, bias, state);
     if (!recorded({&x, &weight}, {&bias, &state})) {
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(seq_conv)>("unetmi::seq_conv");
@@ -467,8 +498,8 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(12);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        joins_capture("selective_scan");
         const variable_list s = ctx->get_saved_variables();
+        joins_capture("selective_scan", s[0]);
         const Tensor dy = grads[0].defined() ? grads[0] : at::zeros_like(s[0], at::MemoryFormat::Contiguous);
         const Maybe dout = grads[1].defined() && grads[1].dim() == 3 ? Maybe(grads[1].contiguous()) : Maybe();
         Wanted wanted{ctx};
@@ -489,6 +520,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
 std::tuple<Tensor, Tensor, Tensor> ssm_scan_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                                                      const Maybe& D, const Maybe& z, const Maybe& dt_bias, const Maybe& state, const Maybe& lengths,
                                                      bool softplus, bool want_state, bool want_marks) {
+    no_tangents("selective_scan", x, dt, A, B, C, D, z, dt_bias, state);
     if (!recorded({&x, &dt, &A, &B, &C}, {&D, &z, &dt_bias, &state})) {       // no node, and no states saved for one
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(ssm_scan)>("unetmi::ssm_scan");
@@ -513,8 +545,8 @@ struct NormNode : torch::autograd::Function<NormNode> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         variable_list out(7);
-        joins_capture("block_norm");
         const variable_list s = ctx->get_saved_variables();
+        joins_capture("block_norm", s[0]);
         const Maybe d_out = grads[0].defined() ? Maybe(grads[0].contiguous()) : Maybe();
         const Maybe d_norm = s[4].defined() && grads[1].defined() ? Maybe(grads[1].contiguous()) : Maybe();
         if (!d_out && !d_norm) return out;
@@ -534,6 +566,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
 };
 std::tuple<Tensor, Tensor, Tensor> block_norm_autograd(const Tensor& x, const Maybe& gate, const Maybe& post, const Maybe& residual,
                                                        const Maybe& scale, const Maybe& pre, double eps, bool want_stats) {
+    no_tangents("block_norm", x, gate, post, residual, scale, pre);
     if (!recorded({&x}, {&gate, &post, &residual, &scale, &pre})) {
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<decltype(block_norm)>("unetmi::block_norm");
@@ -601,7 +634,9 @@ TORCH_LIBRARY_IMPL(unetmi, Autograd, m) {
     m.impl("seq_conv", seq_conv_autograd);
     m.impl("ssm_scan", ssm_scan_autograd);
     m.impl("block_norm", block_norm_autograd);
-    // the tokens' and the backward ops record nothing
-    for (const char* name : {"seq_conv_step", "ssm_scan_step", "seq_conv_bwd", "ssm_scan_bwd", "block_norm_bwd"})
-        m.impl(name, torch::CppFunction::makeFallthrough());
+    m.impl("seq_conv_bwd", Below<kConvBwd, seq_conv_bwd>::call);
+    m.impl("ssm_scan_bwd", Below<kScanBwd, ssm_scan_bwd>::call);
+    m.impl("block_norm_bwd", Below<kNormBwd, block_norm_bwd>::call);
+    m.impl("seq_conv_step", Below<kConvStep, seq_conv_step>::call);
+    m.impl("ssm_scan_step", Below<kScanStep, ssm_scan_step>::call);
 }
