@@ -122,3 +122,23 @@ def test_vmap_takes_samples_one_by_one(ops):
         many = given["x"][None] * torch.arange(1.0, 4.0).reshape((3,) + (1,) * given["x"].dim())
         got = torch.func.vmap(lambda v: call(**{**given, "x": v}))(many)
         assert torch.equal(got, torch.stack([call(**{**given, "x": v}) for v in many])), name
+
+
+def test_token_calls_refuse_to_be_recorded(ops):
+    """Inference only: under grad mode an input, parameter or cache that requires a gradient is refused before the cache is
+    touched; without grad mode, or detached, the same call runs."""
+    for name, call, given in token_calls():
+        for k in given:
+            leaves = {n: t.clone().requires_grad_(n == k) for n, t in given.items()}
+            with pytest.raises(RuntimeError, match=name + " is inference only"):
+                call(**leaves)
+            assert torch.equal(leaves["state"], given["state"])
+            made = {**leaves, k: leaves[k] * 1}                          # no leaf, but part of a graph
+            with pytest.raises(RuntimeError, match=name + " is inference only"):
+                call(**made)
+            with torch.no_grad():
+                y = call(**leaves)
+            assert not y.requires_grad and torch.equal(leaves["state"], given["state"] + 1)
+            with torch.inference_mode():
+                assert torch.equal(call(**leaves), y)
+            assert torch.equal(call(**{n: t.detach() for n, t in leaves.items()}), y)

@@ -427,7 +427,7 @@ template <class... A>
 void no_tangents(const char* what, const A&... args) {
     (no_tangent(what, args), ...);
 }
-// the _bwd and _step ops below the autograd key: they record nothing
+// the _bwd ops below the autograd key: they record nothing
 template <const auto& Name, auto Kernel>
 struct Below;
 template <const auto& Name, class R, class... A, R (*Kernel)(A...)>
@@ -441,6 +441,22 @@ struct Below<Name, Kernel> {
 };
 constexpr char kConvBwd[] = "unetmi::seq_conv_bwd", kScanBwd[] = "unetmi::ssm_scan_bwd", kNormBwd[] = "unetmi::block_norm_bwd",
                kConvStep[] = "unetmi::seq_conv_step", kScanStep[] = "unetmi::ssm_scan_step";
+
+// The token ops write the cache through its pointer and have no gradients.  Where autograd would record the call they say so:
+// a result without a history would cut a training program's gradients off unseen.
+void inference_only(const char* what, std::initializer_list<const Tensor*> given, std::initializer_list<const Maybe*> optional) {
+    TORCH_CHECK(!recorded(given, optional), "unet_amd: ", what, " is inference only, but an input, a parameter or the cache requires a gradient: "
+                "call it under torch.no_grad() or torch.inference_mode(), or on detached tensors");
+}
+Tensor seq_conv_step_autograd(const Tensor& x, const Tensor& weight, const Maybe& bias, const Tensor& state, const Maybe& slots, bool silu) {
+    inference_only("causal_conv_step", {&x, &weight, &state}, {&bias});
+    return Below<kConvStep, seq_conv_step>::call(x, weight, bias, state, slots, silu);
+}
+Tensor ssm_scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Maybe& D, const Maybe& z,
+                              const Maybe& dt_bias, const Tensor& state, const Maybe& slots, bool softplus) {
+    inference_only("selective_scan_step", {&x, &dt, &A, &B, &C, &state}, {&D, &z, &dt_bias});
+    return Below<kScanStep, ssm_scan_step>::call(x, dt, A, B, C, D, z, dt_bias, state, slots, softplus);
+}
 
 struct ConvNode : torch::autograd::Function<ConvNode> {
     static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& bias, const Maybe& state,
@@ -637,6 +653,6 @@ TORCH_LIBRARY_IMPL(unetmi, Autograd, m) {
     m.impl("seq_conv_bwd", Below<kConvBwd, seq_conv_bwd>::call);
     m.impl("ssm_scan_bwd", Below<kScanBwd, ssm_scan_bwd>::call);
     m.impl("block_norm_bwd", Below<kNormBwd, block_norm_bwd>::call);
-    m.impl("seq_conv_step", Below<kConvStep, seq_conv_step>::call);
-    m.impl("ssm_scan_step", Below<kScanStep, ssm_scan_step>::call);
+    m.impl("seq_conv_step", seq_conv_step_autograd);
+    m.impl("ssm_scan_step", ssm_scan_step_autograd);
 }

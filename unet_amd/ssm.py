@@ -49,7 +49,7 @@ def causal_conv(x, weight, bias=None, act=True, state=None, lengths=None, return
 
 
 def causal_conv_step(x, state, weight, bias=None, act=True, slots=None):
-    """One token of every row: x [rows, channels] -> y like x; inference only.
+    """One token of every row: x [rows, channels] -> y like x; inference only (refused where autograd would record it).
 
     state [num_slots, taps-1, channels] is a cache of streams, shifted in place; slots [rows] says which stream a row is
     (without: row i is stream i).  A negative slot is a padding row: zeros out, nothing touched.  A slot beyond the cache,
@@ -72,5 +72,5 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=True, slots=None):
     """One token of every row: x, dt, z [rows, channels], B and C [rows, N] or [rows, groups, N] -> y like x; inference only.
 
-    state [num_slots, channels, N] fp32 is a cache of streams, advanced in place; slots as in causal_conv_step."""
+    state [num_slots, channels, N] fp32 is a cache of streams, advanced in place; slots and gradients as in causal_conv_step."""
     return _ops.ssm_scan_step(x, dt, A, B, C, D, z, dt_bias, state, _index(slots, -1, 2 ** 31 - 1), _flag(softplus, "softplus"))
