@@ -1,6 +1,10 @@
 """How the sequence operators answer automatic differentiation's questions, without a GPU: plain torch stands in for the
 kernels on CPU tensors, everything above them (checks, autograd nodes, refusals) is the package's own."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -142,3 +146,33 @@ def test_token_calls_refuse_to_be_recorded(ops):
             with torch.inference_mode():
                 assert torch.equal(call(**leaves), y)
             assert torch.equal(call(**{n: t.detach() for n, t in leaves.items()}), y)
+
+
+@pytest.mark.parametrize("library", ["missing", "broken"])
+def test_the_package_imports_without_the_sequence_operators(tmp_path, library):
+    """A library that is not there, or does not load, is the sequence operators' trouble alone: the networks import and are
+    built, and the operators say what is missing when they are called."""
+    import unet_amd
+    here, there = os.path.dirname(os.path.abspath(unet_amd.__file__)), tmp_path / "unet_amd"
+    there.mkdir()
+    for name in os.listdir(here):
+        if name.endswith(".py") or name == "libunetmi.so":
+            os.symlink(os.path.join(here, name), there / name)
+    if library == "broken":
+        (there / "libunetmi_torch.so").write_bytes(b"no library")
+    code = """
+import torch, unet_amd
+assert unet_amd.__file__.startswith({!r}), unet_amd.__file__
+unet_amd.UNet(*unet_amd.default_unet_blocks(c_in=2, c_last=1, f_dim=8))
+for call in (lambda: unet_amd.ssm.causal_conv(torch.zeros(1, 4, 8), torch.zeros(8, 4)),
+             lambda: unet_amd.norm.block_norm(torch.zeros(4, 8))):
+    try:
+        call()
+    except ImportError as e:
+        assert "libunetmi_torch.so" in str(e) and "build it" in str(e), e
+    else:
+        raise AssertionError("no refusal")
+print("told")
+""".format(str(tmp_path))
+    done = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, env={**os.environ, "PYTHONPATH": str(tmp_path)})
+    assert done.returncode == 0 and "told" in done.stdout, done.stderr
