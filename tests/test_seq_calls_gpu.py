@@ -1,0 +1,68 @@
+"""Calls of the sequence operators that their own tests leave out: long time axes taken in one piece, strides of axes of one
+element."""
+
+import pytest
+import torch
+
+from seq_oracle import held, scan64
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def rnd(shape, seed, dtype=F32, scale=1.0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def test_parameter_gradients_over_a_long_axis(device):
+    """384 equal sequences of 65536 equal steps, enough blocks for the time axis to stay whole: what dA, dD and ddt_bias add up
+    has one sign, so that a single running sum would be off by up to a rounding a step (thousands here, and to one side).
+    Counted: 1024 terms between two partial sums in memory, 96 + 3 + 32 for the partial sums of 64 pieces of 384 sequences
+    over 32 groups of rows in eights, and for a term 8 roundings each of a state and of an adjoint that forget half of
+    themselves every step, 3 of a decay and a few products."""
+    from unet_amd import ssm
+    B, L = 384, 65536
+    value = dict(x=1.1, dt=0.7, B=0.9, C=1.3, dy=0.7)
+    value = {k: torch.tensor(v, dtype=F32).item() for k, v in value.items()}
+    A, D, bias = -1.0, 0.5, 0.0
+    decay = torch.exp(torch.tensor(value["dt"] * A, dtype=torch.float64)).item()
+    state, states = 0.0, []
+    for _ in range(L):
+        states.append(state)
+        state = decay * state + value["dt"] * value["x"] * value["B"]
+    ahead, dA, dbias, wide = 0.0, 0.0, 0.0, 0.0
+    for before in reversed(states):
+        ahead += value["dy"] * value["C"]
+        du, ahead = ahead * value["B"], ahead * decay
+        w = ahead * before
+        dA += w * value["dt"]
+        dbias += w * A + du * value["x"]
+        wide += abs(w * A) + du * value["x"]
+    row = {k: torch.full((1, L, 1), v, device=device).expand(B, L, 1) for k, v in value.items()}
+    leaves = [torch.full(s, v, device=device).requires_grad_() for s, v in (((1, 1), A), ((1,), D), ((1,), bias))]
+    y = ssm.selective_scan(row["x"], row["dt"], leaves[0], row["B"], row["C"], D=leaves[1], dt_bias=leaves[2], softplus=False)
+    got = torch.autograd.grad(y, leaves, row["dy"])
+    dD = value["dy"] * value["x"] * L
+    for name, g, want, size in zip(("dA", "dD", "ddt_bias"), got, (dA, dD, dbias), (dA, dD, wide)):
+        held(g.reshape(1), torch.tensor([want * B], dtype=torch.float64), torch.tensor([size * B], dtype=torch.float64), 1024 + 131 + 45, name)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_parameter_gradients_of_sequences_that_end_in_different_pieces(device, dtype):
+    """Lengths around the 1024 steps between two partial sums, on a time axis that is not split (384 blocks); what the scratch
+    memory held before does not show."""
+    from unet_amd import ssm
+    B, L, ch, N = 6, 2500, 64, 3
+    lengths = torch.tensor([0, 1, 1023, 1024, 1025, 2500], dtype=torch.int32)
+    g = torch.Generator().manual_seed(3)
+    p = dict(x=rnd((B, L, ch), 1, dtype), dt=rnd((B, L, ch), 2, dtype, 0.7), A=-torch.arange(1.0, N + 1) * (torch.rand((ch, N), generator=g) + 0.5),
+             B=rnd((B, L, ch, N), 3, dtype), C=rnd((B, L, ch, N), 4, dtype), D=rnd((ch,), 5), z=rnd((B, L, ch), 6, dtype), dt_bias=rnd((ch,), 7) - 2)
+    dy = rnd((B, L, ch), 9, dtype)
+    want, room = (scan64(**p, lengths=lengths, dy=dy, magnitude=m) for m in (False, True))
+    leaves = {k: t.to(device).requires_grad_() for k, t in p.items()}
+    y = ssm.selective_scan(**leaves, lengths=lengths.to(device))
+    torch.full((2 ** 26,), float("nan"), device=device)                 # freed at once: the scratch memory comes from here
+    grads = torch.autograd.grad(y, list(leaves.values()), dy.to(device))
+    for k, got in zip(leaves, grads):
+        held(got, want["d_" + k], room["d_" + k], 4 * L + 2 * N + 96 + (B * L if k in ("A", "D", "dt_bias") else 0), "d " + k)

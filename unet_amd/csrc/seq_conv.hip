@@ -335,8 +335,7 @@ __global__ __launch_bounds__(1024) void sum_rows_kernel(const float* __restrict_
             float v[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = rows[(size_t)(r + k * 32) * width + col];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) s += v[k];
+            s += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
         }
         for (; r < R; r += 32) s += rows[(size_t)r * width + col];
     }

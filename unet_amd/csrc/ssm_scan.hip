@@ -26,6 +26,11 @@ template <int S> constexpr int tile_steps() { return S <= 2 ? 32 : 16; }
 template <int S> constexpr int mark_steps() { return S <= 2 ? 16 : S == 4 ? 8 : 4; }
 static int mark_steps_of(int S) { return S <= 2 ? 16 : S == 4 ? 8 : 4; }
 
+// The backward kernel's running sums of dA, dD and ddt_bias go to memory every kPiece steps: a running sum of n terms is off by
+// up to n roundings, and a channel whose time axis is not split would take all its steps in one (65536 steps of equal terms:
+// dA off by 7e-4 of itself, 7e-6 in pieces).
+constexpr int kPiece = 1024;
+
 struct ScanArgs {
     const void *x, *dt, *z, *Bm, *Cm;     // z may be null
     const float *A, *Dp, *bias, *h0;      // Dp, bias, h0 may be null
@@ -33,6 +38,7 @@ struct ScanArgs {
     long long xb, xt, dtb, dtt, zb, zt, bb, bt, bg, cb, ct, cg;      // element strides
     int L, D, N, Dg, tpg;                 // channels per group, blocks per group
     int chunk, nchunk;                    // steps per chunk (a multiple of the tile's)
+    int npiece;                           // kPiece steps per chunk
     int nmark;
     bool softplus;
     void* y;
@@ -43,7 +49,7 @@ struct ScanArgs {
     long long dyb, dyt;
     const float* dhT;
     void *dx, *ddt, *dz;
-    float *dh0, *pBC, *pA;                // partial sums: [B, L, G tpg, 2, 4S]; [B nchunk, (D, 4S), (D), (D)] of A, D, bias
+    float *dh0, *pBC, *pA;                // partial sums: [B, L, G tpg, 2, 4S]; [B nchunk npiece, (D, 4S), (D), (D)] of A, D, bias
 };
 
 struct Place {                            // what a thread works on
@@ -471,8 +477,15 @@ __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs 
                 dst[(size_t)(e / (2 * NP)) * gridDim.x * (2 * NP) + e % (2 * NP)] = (r[e] + r[e + RED]) + (r[e + 2 * RED] + r[e + 3 * RED]);
     };
     float dD = 0.f, dbias = 0.f;
+    auto write_piece = [&](int piece) {                               // its row of partial sums: [D][4S] of A, [D] of D, [D] of ddt_bias
+        const auto part = window(a.pA + (((size_t)p.b * a.nchunk + chunk) * a.npiece + piece) * a.D * (NP + 2));
+        window_store_states<S>(dA, part, p.live ? (p.ch * NP + p.q * S) * 4 : kOutside);
+        const float sum_D = quad_sum(dD), sum_bias = quad_sum(dbias);
+        window_store<float>(p.q == 0 ? sum_D : sum_bias, part, p.live && p.q < 2 ? (a.D * (NP + p.q) + p.ch) * 4 : kOutside, 0);
+    };
+    for (int piece = (max(left, 0) + kPiece - 1) / kPiece; piece < a.npiece; ++piece) write_piece(piece);      // behind the end: zeros
     int half = 0, before = -1;                                        // before: the tile whose sums wait in the other half
-    for (; dt0 >= 0; dt0 -= MK, half ^= 1) {
+    auto tile = [&] {
         float *lb = lds_b[half], *lc = lds_c[half];
         bs.store(lb);
         cs.store(lc);
@@ -579,19 +592,18 @@ __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs 
                 vc.store(r + m * 2 * NP + NP);
             }
         }
+    };
+    while (dt0 >= 0) {
+        const int piece = dt0 / kPiece;
+        for (; dt0 >= piece * kPiece; dt0 -= MK, half ^= 1) tile();
+        write_piece(piece);
+#pragma unroll
+        for (int s = 0; s < S; ++s) dA[s] = 0.f;
+        dD = dbias = 0.f;
     }
     __syncthreads();
     if (before >= 0) write_sums(before, red[half ^ 1]);
-    dD = quad_sum(dD);
-    dbias = quad_sum(dbias);
     if (!p.live) return;
-    float* part = a.pA + ((size_t)p.b * a.nchunk + chunk) * a.D * (NP + 2);
-#pragma unroll
-    for (int s = 0; s < S; ++s) part[(size_t)p.ch * NP + p.q * S + s] = dA[s];
-    if (p.q == 0) {
-        part[(size_t)a.D * NP + p.ch] = dD;
-        part[(size_t)a.D * (NP + 1) + p.ch] = dbias;
-    }
     if (chunk == 0 && a.dh0) store_states<S>(g, a.dh0 + ((size_t)p.b * a.D + p.ch) * a.N, p.q, a.N);
     for (int t = max(t0, tend) + p.q; t < t1; t += 4) {                // behind the sequence's end
         const size_t o = ((size_t)p.b * a.L + t) * a.D + p.ch;
@@ -697,7 +709,7 @@ namespace {
 int lane_states(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 
 struct ScanPlan {
-    int S, NP, tpg, nchunk, chunk, nmark;
+    int S, NP, tpg, nchunk, chunk, npiece, nmark;
 };
 
 // Time is split where the blocks of the batch's channels alone do not fill the chip's 256 CUs: the first pass over the
@@ -725,6 +737,7 @@ ScanPlan scan_plan(const UnetmiScanDesc& d, bool ragged, bool backward) {
     if (p.chunk < kAlign) p.chunk = kAlign;
     p.nchunk = (d.length + p.chunk - 1) / p.chunk;
     if (p.nchunk < 1) p.nchunk = 1;
+    p.npiece = (p.chunk + kPiece - 1) / kPiece;
     const int mk = mark_steps_of(p.S);
     p.nmark = (d.length + mk - 1) / mk;
     return p;
@@ -759,7 +772,7 @@ ScanArgs scan_args(const UnetmiScanDesc& d, const ScanPlan& p, const void* x, co
     a.bb = d.b_stride[0]; a.bt = d.b_stride[1]; a.bg = d.b_stride[2];
     a.cb = d.c_stride[0]; a.ct = d.c_stride[1]; a.cg = d.c_stride[2];
     a.L = d.length; a.D = d.channels; a.N = d.state; a.Dg = d.channels / d.groups; a.tpg = p.tpg;
-    a.chunk = p.chunk; a.nchunk = p.nchunk; a.nmark = p.nmark; a.softplus = d.softplus != 0;
+    a.chunk = p.chunk; a.nchunk = p.nchunk; a.npiece = p.npiece; a.nmark = p.nmark; a.softplus = d.softplus != 0;
     return a;
 }
 
@@ -812,7 +825,7 @@ struct RunScanBwd {
                                static_cast<T*>(dC), a.lengths, rows, d.length, d.groups, p.tpg, d.state, p.NP);
             if ((rc = launched("ssm_scan_bwd B C")) != UNETMI_OK) return rc;
         }
-        return launch_sum_rows(a.pA, d.batch * p.nchunk, {dA, d.channels * p.NP, p.NP, d.state}, {dD, d.channels, 1, 1},
+        return launch_sum_rows(a.pA, d.batch * p.nchunk * p.npiece, {dA, d.channels * p.NP, p.NP, d.state}, {dD, d.channels, 1, 1},
                                {dbias, d.channels, 1, 1}, s);
     }
 };
@@ -869,7 +882,7 @@ int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
 size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d, int ragged) {
     if (scan_check(d, "ssm_scan_bwd_workspace_bytes") != UNETMI_OK) return 0;
     const ScanPlan p = scan_plan(*d, ragged != 0, true);
-    const size_t parts = (size_t)d->batch * p.nchunk;
+    const size_t parts = (size_t)d->batch * p.nchunk * p.npiece;
     return (summary_floats(*d, p) + (size_t)d->batch * d->length * d->groups * p.tpg * 2 * p.NP + parts * d->channels * (p.NP + 2)) * sizeof(float);
 }
 
@@ -888,11 +901,11 @@ int unetmi_ssm_scan_bwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
     ScanArgs a = scan_args(*d, p, x, dt, A, B, C, D, z, dt_bias);
     a.lengths = lengths; a.marks = const_cast<float*>(marks);
     a.dy = dy; a.dhT = dstate_out; a.dx = dx; a.ddt = ddt; a.dz = dz; a.dh0 = dstate;
-    const size_t parts = (size_t)d->batch * p.nchunk;
+    const size_t chunks = (size_t)d->batch * p.nchunk;
     a.hend = static_cast<float*>(ws);                                 // multiples of four floats first: they stay 16-byte aligned
-    a.pBC = a.hend + (p.nchunk > 1 ? parts * d->channels * p.NP : 0);
+    a.pBC = a.hend + (p.nchunk > 1 ? chunks * d->channels * p.NP : 0);
     a.pA = a.pBC + (size_t)d->batch * d->length * d->groups * p.tpg * 2 * p.NP;
-    a.sdt = a.pA + parts * d->channels * (p.NP + 2);
+    a.sdt = a.pA + chunks * p.npiece * d->channels * (p.NP + 2);
     return scan_dispatch<RunScanBwd>(*d, p.S, *d, p, a, dB, dC, dA, dD, ddt_bias, static_cast<hipStream_t>(stream));
 }
 
