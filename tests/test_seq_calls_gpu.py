@@ -66,3 +66,19 @@ def test_parameter_gradients_of_sequences_that_end_in_different_pieces(device, d
     grads = torch.autograd.grad(y, list(leaves.values()), dy.to(device))
     for k, got in zip(leaves, grads):
         held(got, want["d_" + k], room["d_" + k], 4 * L + 2 * N + 96 + (B * L if k in ("A", "D", "dt_bias") else 0), "d " + k)
+
+
+def test_norm_weight_gradients_over_many_rows(device):
+    """2^26 equal rows: a weight's gradient adds up terms of one sign.  Counted: 1024 rows between two partial sums in memory,
+    256 + 3 + 32 for the partial sums of 65536 threads' rows over 32 groups of rows in eights, 64 for a term (a mean over a row
+    and a few products)."""
+    from unet_amd import norm
+    rows, D = 2 ** 26, 8
+    x = torch.linspace(0.6, 1.7, D, dtype=F32)
+    w, dy = torch.linspace(0.9, 1.3, D, dtype=F32), torch.linspace(0.7, 1.9, D, dtype=F32)
+    leaf = w.to(device).requires_grad_()
+    p = norm.block_norm(x.to(device).expand(rows, D), post_weight=leaf)
+    got, = torch.autograd.grad(p, leaf, dy.to(device).expand(rows, D))
+    v = x.double() * torch.rsqrt(x.double().pow(2).mean() + 1e-6)
+    want = rows * dy.double() * v
+    held(got, want, want.abs(), 1024 + 291 + 64, "d post_weight")

@@ -285,11 +285,13 @@ NormPlan norm_plan(const UnetmiNormDesc& d, long long most_blocks) {
 long long fwd_blocks(const UnetmiNormDesc& d) { const NormPlan p = norm_plan(d, 1); return 256 * 64 / (p.width * p.per_block / 64); }
 // Backward: whole blocks a CU, all resident (every block more costs 12 bytes a column of partial sums, and 1.2 blocks a CU take
 // as long as two), sixteen waves of them with 16-bit activations and eight with fp32, whose rows are twice the bytes: 16387 x 2048
-// bf16 145, 119 and 110 us with 8, 12 and 16 waves, 16032 x 1285 bf16 194, 127 and 115, fp32 139, 151 and 156.
+// bf16 145, 119 and 110 us with 8, 12 and 16 waves, 16032 x 1285 bf16 194, 127 and 115, fp32 139, 151 and 156.  More where a
+// thread would add up more than 1024 rows of the weights' gradients in one running sum, which may be off by a rounding a row.
 long long bwd_blocks(const UnetmiNormDesc& d) {
     const NormPlan p = norm_plan(d, 1);
     const int per_cu = (d.dtype == UNETMI_DTYPE_BF16 ? 16 : 8) / (p.width * p.per_block / 64);
-    return 256 * (per_cu ? per_cu : 1);
+    const long long resident = 256 * (per_cu ? per_cu : 1), long_sums = (d.rows + 1024 * p.per_block - 1) / (1024 * p.per_block);
+    return resident > long_sums ? resident : long_sums;
 }
 
 int norm_check(const UnetmiNormDesc* d, const char* what) {
