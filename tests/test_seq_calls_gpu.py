@@ -82,3 +82,48 @@ def test_norm_weight_gradients_over_many_rows(device):
     v = x.double() * torch.rsqrt(x.double().pow(2).mean() + 1e-6)
     want = rows * dy.double() * v
     held(got, want, want.abs(), 1024 + 291 + 64, "d post_weight")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_of_single_entries(device, dtype):
+    """An axis of one element may have any stride (a prompt of one step out of a time-major buffer: the whole batch lies between
+    two steps): the same as dense inputs, bit for bit."""
+    from unet_amd import norm, ssm
+    far = 2 ** 25
+
+    def spread(t, axes):
+        """The same values with the given strides on axes of one element."""
+        strides = list(t.stride())
+        for a in axes:
+            assert t.shape[a] == 1
+            strides[a] = far
+        return t.as_strided(t.shape, strides)
+
+    B, C, N = 3, 72, 5
+    A = (-torch.rand((C, N), generator=torch.Generator().manual_seed(1)) - 0.1).to(device)
+    w = rnd((C, 4), 2).to(device)
+    x, dt, z, dy = (rnd((B, 1, C), 3 + i, dtype).to(device) for i in range(4))
+    b, c = rnd((B, 1, N), 7, dtype).to(device), rnd((B, 1, 1, N), 8, dtype).to(device)
+    grouped = b.view(B, 1, 1, N)
+
+    def scan(move):
+        leaves = [move(t, (1,)).detach().requires_grad_() for t in (x, dt, z)] + [move(grouped, (1, 2)).detach().requires_grad_(),
+                                                                                 move(c, (1, 2)).detach().requires_grad_()]
+        y = ssm.selective_scan(leaves[0], leaves[1], A, leaves[3], leaves[4], z=leaves[2])
+        return (y,) + torch.autograd.grad(y, leaves, move(dy, (1,)))
+
+    def conv(move):
+        leaf = move(x, (1,)).detach().requires_grad_()
+        y = ssm.causal_conv(leaf, w)
+        return (y,) + torch.autograd.grad(y, leaf, move(dy, (1,)))
+
+    def tokens(move):
+        state, cache = torch.ones(1, C, N, device=device), torch.ones(1, 3, C, device=device, dtype=dtype)
+        row = lambda t, axes: move(t[:1, 0], axes)  # noqa: E731
+        return (ssm.selective_scan_step(row(x, (0,)), row(dt, (0,)), A, row(b, (0,)), row(b, (0,)), state, z=row(z, (0,))),
+                ssm.causal_conv_step(row(x, (0,)), cache, w), state, cache,
+                norm.block_norm(row(x, (0,)), gate=row(z, (0,)), residual=row(dy, (0,))))
+
+    for call in (scan, conv, tokens):
+        with torch.set_grad_enabled(call is not tokens):
+            assert all(torch.equal(a, b) for a, b in zip(call(lambda t, axes: t), call(spread))), call.__name__

@@ -76,10 +76,13 @@ void dense(const Maybe& t, const char* name, const char* op, at::ScalarType type
     if (t) dense(*t, name, op, type, like, shape);
 }
 
+// elements between two entries of an axis; a single entry's stride may be anything and means nothing
+int64_t apart(const Tensor& t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
+
 // the last axis dense and steps not too far apart: a copy where they are not
 Tensor rows(const Tensor& t) {
     const int64_t n = t.dim();
-    const bool ok = (t.stride(n - 1) == 1 || t.size(n - 1) <= 1) && (n < 3 || t.stride(1) <= UNETMI_SEQ_MAX_STEP);
+    const bool ok = (t.stride(n - 1) == 1 || t.size(n - 1) <= 1) && (n < 3 || apart(t, 1) <= UNETMI_SEQ_MAX_STEP);
     return ok ? t : t.contiguous();
 }
 
@@ -120,7 +123,7 @@ std::tuple<Tensor, Tensor> seq_conv(const Tensor& x0, const Tensor& weight, cons
                                     bool want_state) {
     UnetmiSeqConvDesc d = conv_desc("seq_conv", x0, weight, bias, state, lengths, silu);
     const Tensor x = rows(x0);
-    d.x_stride[0] = x.stride(0); d.x_stride[1] = x.stride(1);
+    d.x_stride[0] = apart(x, 0); d.x_stride[1] = apart(x, 1);
     const c10::DeviceGuard guard(x.device());
     const Tensor y = empty(x.sizes(), x);
     const Tensor out = want_state ? empty({d.batch, d.taps - 1, d.channels}, x) : empty({0}, x);
@@ -137,8 +140,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> seq_conv_bwd(const Tensor& x0, const 
     same(dy0, "dy", op, x0.scalar_type(), x0, x0.sizes());
     dense(dstate_out, "dstate_out", op, x0.scalar_type(), x0, {d.batch, d.taps - 1, d.channels});
     const Tensor x = rows(x0), dy = rows(dy0);
-    d.x_stride[0] = x.stride(0); d.x_stride[1] = x.stride(1);
-    d.dy_stride[0] = dy.stride(0); d.dy_stride[1] = dy.stride(1);
+    d.x_stride[0] = apart(x, 0); d.x_stride[1] = apart(x, 1);
+    d.dy_stride[0] = apart(dy, 0); d.dy_stride[1] = apart(dy, 1);
     const c10::DeviceGuard guard(x.device());
     const Tensor dx = empty(x.sizes(), x), dw = empty(weight.sizes(), weight), db = empty({d.channels}, weight);
     const Tensor dstate = state ? empty(state->sizes(), x) : empty({0}, x);
@@ -167,7 +170,7 @@ Tensor seq_conv_step(const Tensor& x0, const Tensor& weight, const Maybe& bias, 
     d.batch = count(B, op); d.length = 1; d.channels = count(D, op); d.taps = count(K, op);
     const Tensor x = rows(x0);
     d.act = silu ? UNETMI_ACT_SILU : UNETMI_ACT_NONE;
-    d.x_stride[0] = x.stride(0);
+    d.x_stride[0] = apart(x, 0);
     const c10::DeviceGuard guard(x.device());
     const Tensor y = empty(x.sizes(), x);
     check(lib.conv_step(&d, ptr(x), f32(weight), f32(bias), i32(slots), slot_count, ptr(state), ptr(y), stream_of(x)), "unetmi_seq_conv_step");
@@ -205,10 +208,10 @@ struct ScanIn {
         if (z0) z = rows(*z0);
         d.softplus = softplus;
         for (int64_t i = 0; i < axes - 1; ++i) {
-            d.x_stride[i] = x.stride(i); d.dt_stride[i] = dt.stride(i); d.z_stride[i] = z ? z->stride(i) : 0;
-            d.b_stride[i] = B.stride(i); d.c_stride[i] = C.stride(i);
+            d.x_stride[i] = apart(x, i); d.dt_stride[i] = apart(dt, i); d.z_stride[i] = z ? apart(*z, i) : 0;
+            d.b_stride[i] = apart(B, i); d.c_stride[i] = apart(C, i);
         }
-        if (grouped) { d.b_stride[2] = B.stride(axes - 1); d.c_stride[2] = C.stride(axes - 1); }
+        if (grouped) { d.b_stride[2] = apart(B, axes - 1); d.c_stride[2] = apart(C, axes - 1); }
     }
 };
 
@@ -249,7 +252,7 @@ Nine ssm_scan_bwd(const Tensor& x0, const Tensor& dt0, const Tensor& A, const Te
     dense(dstate_out, "dstate_out", op, at::kFloat, x, {d.batch, d.channels, d.state});
     dense(marks, "marks", op, at::kFloat, x, {(int64_t)(lib.scan_marks_bytes(&d) / sizeof(float))});
     const Tensor dy = rows(dy0);
-    d.dy_stride[0] = dy.stride(0); d.dy_stride[1] = dy.stride(1);
+    d.dy_stride[0] = apart(dy, 0); d.dy_stride[1] = apart(dy, 1);
     const c10::DeviceGuard guard(x.device());
     const Tensor dx = empty(x.sizes(), x), ddt = empty(x.sizes(), x), dB = empty(in.B.sizes(), x), dC = empty(in.B.sizes(), x);
     const Tensor dz = in.z ? empty(x.sizes(), x) : empty({0}, x);
@@ -304,15 +307,15 @@ struct NormIn {
         if (gate0) {
             same(*gate0, "gate", op, x0.scalar_type(), x0, shape);
             gate = rows(*gate0);
-            d.gate_stride = gate->stride(0);
+            d.gate_stride = apart(*gate, 0);
         }
         if (residual0) {
             residual_type = residual0->scalar_type() == at::kFloat ? at::kFloat : x0.scalar_type();
             same(*residual0, "residual", op, residual_type, x0, shape);
             residual = rows(*residual0);
-            d.residual_stride = residual->stride(0);
+            d.residual_stride = apart(*residual, 0);
         }
-        d.rows = shape[0]; d.channels = count(shape[1], op); d.eps = eps; d.x_stride = x.stride(0);
+        d.rows = shape[0]; d.channels = count(shape[1], op); d.eps = eps; d.x_stride = apart(x, 0);
         d.residual_dtype = residual_type == at::kBFloat16 ? UNETMI_DTYPE_BF16 : UNETMI_DTYPE_F32;
     }
 };
