@@ -579,7 +579,8 @@ int unetmi_seq_conv_step(const UnetmiSeqConvDesc* d, const void* x, const float*
  * g*channels/groups .. of group g; D, dt_bias [channels]; D, z, dt_bias may be NULL.  State [batch, channels, state] fp32
  * (NULL: zeros); state_out may be NULL and must not be `state`.  The inputs' steps are at most UNETMI_SEQ_MAX_STEP elements
  * apart.  marks (NULL for inference): the states that the backward
- * call starts its tiles from, unetmi_ssm_scan_marks_bytes of them.  States, decays and sums are fp32 throughout. */
+ * call starts its tiles from, unetmi_ssm_scan_marks_bytes of them (8 bytes a sequence, step and channel with 16 states, 64 with
+ * 64).  States, decays and sums are fp32 throughout. */
 #define UNETMI_SEQ_MAX_STEP (1 << 24)
 typedef struct UnetmiScanDesc {
     int32_t batch, length, channels, state, groups, dtype, softplus, reserved;
@@ -593,7 +594,8 @@ int unetmi_ssm_scan_fwd(const UnetmiScanDesc* d, const void* x, const void* dt, 
                         const float* D, const void* z, const float* dt_bias, const float* state, const int32_t* lengths, void* y,
                         float* state_out, float* marks, void* ws, size_t ws_bytes, void* stream);
 
-/* Gradients of unetmi_ssm_scan_fwd from the marks of that call.  dD and ddt_bias are written
+/* Gradients of unetmi_ssm_scan_fwd from the marks of that call.  The workspace holds a partial sum of dB and dC for every step
+ * and block of 64 channels of a group: many narrow groups make it large.  dD and ddt_bias are written
  * also without D and dt_bias.  dstate_out: the final state's gradient or NULL; dstate: the initial state's, or NULL.  Sums over channels
  * and sequences are taken in a fixed order: equal calls give equal bits. */
 size_t unetmi_ssm_scan_bwd_workspace_bytes(const UnetmiScanDesc* d, int ragged);

@@ -6,9 +6,10 @@
 // Rows are read once and written once (three inputs, two outputs: ten bytes a bfloat16 element, about 16 operations), so
 // HBM bounds both directions.  A thread holds eight elements of a row in fp32: rows of up to 512 elements are one wave, wider
 // ones a block of up to sixteen.  Blocks walk over rows.  Forward, the weights stay in registers; backward in LDS (a wave a SIMD
-// more, and rows of 8192 without spills: 4096 x 8192 bf16 299 -> 114 us), the weights' gradients as partial sums in registers,
-// added up in a fixed order by a second kernel.  Measured: forward 16387 x 2048 bf16 61 us (5.5 TB/s), 16032 x 1285 fp32 80 us
-// (5.1 TB/s), backward 110 us (4.9 TB/s) and 139 us (4.7 TB/s) and 5 for the sums; 64 rows of 2048 in 4 us.
+// more, and bfloat16 rows of 8192 without spills: 4096 x 8192 299 -> 114 us; fp32 rows above 4096, at the 128 registers that a
+// block of 1024 threads leaves, still spill 18: 4096 x 8192 221 us, 4.9 TB/s), the weights' gradients as partial sums in
+// registers, added up in a fixed order by a second kernel.  Measured (medians): forward 16387 x 2048 bf16 63 us (5.3 TB/s),
+// 16032 x 1285 fp32 77 us (5.3 TB/s), backward 111 us (4.8 TB/s) and 139 us (4.7 TB/s) and 5 for the sums; 64 rows of 2048 in 4 us.
 #include "seq_common.hpp"
 
 #include <type_traits>

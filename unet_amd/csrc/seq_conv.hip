@@ -5,8 +5,8 @@
 // keeps four channels and walks along time with the last K-1 inputs in registers, so a row is read once per time segment plus
 // K-1 rows that the caches still hold.  Four also of 16 bits, 512 bytes a wave and row: eight take so many registers that two
 // waves a SIMD remain of four (8 x 4096 x 2048 bf16 forward 54 -> 47 us, backward 113 -> 98; 32 x 501 x 768 13.8 -> 11.1 and 31
-// -> 27).  Measured: forward 32 x 501 x 768 fp32 20 us (4.9 TB/s), 8 x 4096 x 2048 bf16 of lengths 0..4096 41 us; backward of
-// the former 36 us (4.1 TB/s) and 4 for the sums; 256 tokens x 2048 channels bf16 4 us.
+// -> 27).  Measured (medians): forward 32 x 501 x 768 fp32 20 us (4.9 TB/s), 8 x 4096 x 2048 bf16 of lengths 0..4096 40 us;
+// backward of the former 36 us (4.1 TB/s) and 4 for the sums; 256 tokens x 2048 channels bf16 4 us.
 #include "seq_common.hpp"
 
 namespace unetmi {
@@ -19,7 +19,7 @@ struct ConvSeqArgs {
     const float *w, *bias;             // [D, K], [D] or null
     const void* state;                 // [B, K-1, D] or null
     const int* lengths;                // [B] or null
-    int B, L, D, act;
+    int B, L, D;
     int steps;                         // time steps per thread
     int cw_log2;                       // threads along the channel vectors = 1 << cw_log2
 };
@@ -399,7 +399,7 @@ ConvSeqArgs conv_args(const UnetmiSeqConvDesc& d, const ConvSeqPlan& p, const vo
     ConvSeqArgs a;
     a.x = x; a.xb = d.x_stride[0]; a.xt = d.x_stride[1];
     a.w = w; a.bias = bias; a.state = state; a.lengths = lengths;
-    a.B = d.batch; a.L = d.length; a.D = d.channels; a.act = d.act;
+    a.B = d.batch; a.L = d.length; a.D = d.channels;
     a.steps = p.steps; a.cw_log2 = p.cw_log2;
     return a;
 }

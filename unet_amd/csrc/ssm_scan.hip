@@ -15,11 +15,11 @@
 
 namespace unetmi {
 
-constexpr int kAlign = 16;                // chunks of the time axis start at multiples of this
+constexpr int kAlign = 16;                // chunks of the time axis start at multiples of this, itself one of every mark_steps
 constexpr int kCh = 64;                   // channels per block
 
 // Steps per tile of the forward kernels: a tile's computation has to cover the next one's loads, and with few states a step
-// is short (16 x 1024 x 2048 bf16: 137 us for 4 and 140 for 8 states with 32 steps, 186 and 196 with 16; 16 states: 99 and 95).
+// is short (16 x 1024 x 2048 bf16: 138 us for 4 and 148 for 8 states with 32 steps, 186 and 196 with 16; 16 states: 207 and 202).
 template <int S> constexpr int tile_steps() { return S <= 2 ? 32 : 16; }
 
 // steps between two saved states, = the steps the backward kernel keeps in registers
@@ -37,7 +37,7 @@ struct ScanArgs {
     const int* lengths;
     long long xb, xt, dtb, dtt, zb, zt, bb, bt, bg, cb, ct, cg;      // element strides
     int L, D, N, Dg, tpg;                 // channels per group, blocks per group
-    int chunk, nchunk;                    // steps per chunk (a multiple of the tile's)
+    int chunk, nchunk;                    // steps per chunk: a multiple of kAlign; its last tile may hold fewer steps than a tile's
     int npiece;                           // kPiece steps per chunk
     int nmark;
     bool softplus;
@@ -204,8 +204,8 @@ __device__ __forceinline__ float at(const void* p, long long i) { return widen(s
 // sum of its steps (the product of its decays is exp(A sum dt)).  Else the whole operator on a chunk, starting from the
 // states of the chunks before it; kMarks also saves the states that the backward kernel starts its tiles from.  A tile's
 // inputs are loaded while the tile before it is computed, B and C go into the other half of LDS: one barrier a tile.
-// Measured: 1 x 8192 x 2048 channels x 16 states bf16 58 + 88 us in 32 chunks, the vector units 88 and 81 % busy with 22 and
-// 33 instructions a step and wave; 128 x 501 x 256 fp32 with marks 110 us (3.6 TB/s); 4 x 4096 x 2048 bf16 110 + 181 us.
+// Measured (medians): 1 x 8192 x 2048 channels x 16 states bf16 62 + 95 us in 32 chunks, the vector units 87 and 86 % busy with
+// 23 and 34 instructions a step and wave; 128 x 501 x 256 fp32 with marks 122 us (3.2 TB/s); 4 x 4096 x 2048 bf16 117 + 190 us.
 enum ScanPass { kStates, kOutputs, kMarks };
 
 template <class T, int S, ScanPass PASS>
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanArgs a) {
 
 // The first backward pass over a split time axis: the adjoint that a chunk hands to the chunk before it, from zero,
 // and the sum of its steps.  Built like the forward pass, from the chunk's last tile to its first.  4 x 4096 x 2048 bf16 in
-// eight chunks: 125 us, vector units 90 % busy.
+// eight chunks: 132 us, vector units 90 % busy.
 template <class T, int S>
 __global__ __launch_bounds__(256) void scan_bwd_state_kernel(ScanArgs a) {
     constexpr int NP = 4 * S, kTile = tile_steps<S>();
@@ -429,9 +429,11 @@ __device__ __forceinline__ void channel_sums(float (&v)[MK][S]) {
 // A channel's shares of dB and dC take the registers of its a_t and h_t; they are summed over the wave by lane exchanges
 // and over the block's waves through LDS, and the block writes one row of partial sums per step.  One barrier a tile: the
 // LDS areas are used in turn, and a tile's sums are taken after the next one's barrier.  Tiles of eight steps (16 states)
-// keep the kernel at 191 registers and two waves a SIMD; sixteen steps spilled there (817 us for 128 x 501 x 256 fp32) and
-// took 357 us at one wave.  Measured: 255 us there, 470 us for 4 x 4096 x 2048 bf16, vector units 82 and 86 % busy with 98
-// instructions a step and wave (16 of them the exchanges; the same sums as fp32 matrix products took 373 and 694 us).
+// keep the kernel at 193 registers and two waves a SIMD; sixteen steps spilled there (817 us for 128 x 501 x 256 fp32 where
+// eight took 257) and took 357 us at one wave.  33 to 64 states take all 256 registers and 81 accumulation registers, one wave a
+// SIMD, and spill 4.  Measured (medians): 285 us there, 499 us for 4 x 4096 x 2048 bf16, vector units 83 and 88 % busy with 100
+// instructions a step and wave (16 of them the exchanges; the same sums as fp32 matrix products took 373 and 694 us where these
+// took 257 and 473); 8 x 2048 x 2048 bf16 251 us with 4 states, 818 with 32, 2140 with 64.
 template <class T, int S>
 __global__ __launch_bounds__(256, S <= 8 ? 2 : 1) void scan_bwd_kernel(ScanArgs a) {
     constexpr int NP = 4 * S, MK = mark_steps<S>(), NI = MK / 4, RED = MK * 2 * NP;
@@ -631,7 +633,8 @@ __global__ __launch_bounds__(256) void scan_bc_kernel(const float* __restrict__ 
 }
 
 // The token kernel's lanes take their states four at a time, so that a quad's accesses are 64 bytes in a row, and as vectors
-// for any number of states (256 x 2048: 64 states 62 -> 48 us, 61 states 114 -> 51).
+// for any number of states (256 x 2048, one cache over and over: 64 states 62 -> 48 us, 61 states 114 -> 51; on caches that HBM
+// has to bring, 75 and 89).
 template <int S>
 __device__ __forceinline__ int token_state(int q, int s) { return S <= 4 ? q * S + s : s / 4 * 16 + q * 4 + s % 4; }
 template <int S>
@@ -713,12 +716,13 @@ struct ScanPlan {
 };
 
 // Time is split where the blocks of the batch's channels alone do not fill the chip's 256 CUs: the first pass over the
-// chunks costs about 0.6 of the second, so it does not pay before (128 sequences of 501 steps, 512 blocks: 104 us in one
-// chunk, 35 + 94 us in two; 1 x 8192 steps x 2048 channels, 32 blocks: 99 + 64 us in 16 chunks, 90 + 60 in 32, 98 + 58 in
+// chunks costs about 0.6 of the second, so it does not pay before (128 sequences of 501 steps, 512 blocks: 115 us in one
+// chunk, 36 + 99 us in two; 1 x 8192 steps x 2048 channels, 32 blocks: 66 + 103 us in 16 chunks, 64 + 97 in 32, 65 + 111 in
 // 64).  With up to 8 states, where a step is short and one wave a SIMD waits for its loads, a split still pays at 256 blocks
-// (8 x 2048 x 2048 x 4: 227 us in one chunk, 177 in four).  The backward kernel, two blocks a CU, gains from a split up to
+// (8 x 2048 x 2048 x 4: 215 us in one chunk, 57 + 127 in four).  The backward kernel, two blocks a CU, gains from a split up to
 // 384 blocks.  Sequences that end early (`ragged`) leave their last chunks empty, and finer chunks even that out (8 x 2001 x
-// 1280: 195 us in 3 chunks, 156 in 6, 122 in 21).
+// 1280, 26 chunks by this rule: 197 us in 3 chunks, 163 in 6, 126 in 21, 135 in 26).  Blocks do not span groups: a group of
+// fewer than 64 channels leaves lanes idle, and counts here as if it did not.
 ScanPlan scan_plan(const UnetmiScanDesc& d, bool ragged, bool backward) {
     ScanPlan p;
     p.S = lane_states(d.state);
