@@ -35,7 +35,9 @@ class Tree:
         return subprocess.run(["make", "-C", str(self.csrc), "PYTHON={}".format(self.root / "python"), *args], capture_output=True, text=True)
 
     def stale(self, target, *settings):
-        return self.make("-q", target, *settings).returncode == 1
+        answer = self.make("-q", target, *settings)
+        assert answer.returncode in (0, 1), answer.stderr
+        return answer.returncode == 1
 
     def compiled(self, *settings):
         """The commands that would compile kernels."""

@@ -169,10 +169,10 @@ for call in (lambda: unet_amd.ssm.causal_conv(torch.zeros(1, 4, 8), torch.zeros(
     try:
         call()
     except ImportError as e:
-        assert "libunetmi_torch.so" in str(e) and "build it" in str(e), e
+        assert "libunetmi_torch.so" in str(e) and "build it" in str(e) and {!r} in str(e), e
     else:
         raise AssertionError("no refusal")
 print("told")
-""".format(str(tmp_path))
+""".format(str(tmp_path), "missing" if library == "missing" else "file too short")
     done = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, env={**os.environ, "PYTHONPATH": str(tmp_path)})
     assert done.returncode == 0 and "told" in done.stdout, done.stderr

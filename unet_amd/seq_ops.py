@@ -25,7 +25,7 @@ def _load():
     try:
         torch.ops.load_library(TORCH_LIB_PATH)
     except OSError as e:                                  # built against another torch, say
-        return "{} does not load ({}) -- {}".format(TORCH_LIB_PATH, e, again)
+        return "{} does not load ({}) -- {}".format(TORCH_LIB_PATH, e.__cause__ or e, again)
     if ctypes.CDLL(TORCH_LIB_PATH).unetmi_torch_bind(os.fsencode(_lib.LIB_PATH)) != 0:
         raise ImportError("unet_amd: {} does not export the sequence operators".format(_lib.LIB_PATH))
     return None
