@@ -12,6 +12,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <torch/types.h>
@@ -428,18 +429,18 @@ void no_tangent(const char* what, const Maybe& t) {
 }
 template <class... A>
 void no_tangents(const char* what, const A&... args) {
-    (no_tangent(what, args), ...);
+    if (torch::autograd::ForwardADLevel::try_get_by_idx(0)) (no_tangent(what, args), ...);         // tangents live inside a level
 }
-// the _bwd ops below the autograd key: they record nothing
+// the _bwd and _step ops below the autograd key: they record nothing
 template <const auto& Name, auto Kernel>
 struct Below;
 template <const auto& Name, class R, class... A, R (*Kernel)(A...)>
 struct Below<Name, Kernel> {
-    static R call(A... args) {
+    static R call(c10::DispatchKeySet keys, A... args) {
         no_tangents(Name, args...);
         at::AutoDispatchBelowADInplaceOrView below;
         static auto op = typed<R(A...)>(Name);
-        return op.call(args...);
+        return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, args...);
     }
 };
 constexpr char kConvBwd[] = "unetmi::seq_conv_bwd", kScanBwd[] = "unetmi::ssm_scan_bwd", kNormBwd[] = "unetmi::block_norm_bwd",
@@ -451,14 +452,15 @@ void inference_only(const char* what, std::initializer_list<const Tensor*> given
     TORCH_CHECK(!recorded(given, optional), "unet_amd: ", what, " is inference only, but an input, a parameter or the cache requires a gradient: "
                 "call it under torch.no_grad() or torch.inference_mode(), or on detached tensors");
 }
-Tensor seq_conv_step_autograd(const Tensor& x, const Tensor& weight, const Maybe& bias, const Tensor& state, const Maybe& slots, bool silu) {
+Tensor seq_conv_step_autograd(c10::DispatchKeySet keys, const Tensor& x, const Tensor& weight, const Maybe& bias, const Tensor& state,
+                              const Maybe& slots, bool silu) {
     inference_only("causal_conv_step", {&x, &weight, &state}, {&bias});
-    return Below<kConvStep, seq_conv_step>::call(x, weight, bias, state, slots, silu);
+    return Below<kConvStep, seq_conv_step>::call(keys, x, weight, bias, state, slots, silu);
 }
-Tensor ssm_scan_step_autograd(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Maybe& D, const Maybe& z,
-                              const Maybe& dt_bias, const Tensor& state, const Maybe& slots, bool softplus) {
+Tensor ssm_scan_step_autograd(c10::DispatchKeySet keys, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                              const Maybe& D, const Maybe& z, const Maybe& dt_bias, const Tensor& state, const Maybe& slots, bool softplus) {
     inference_only("selective_scan_step", {&x, &dt, &A, &B, &C, &state}, {&D, &z, &dt_bias});
-    return Below<kScanStep, ssm_scan_step>::call(x, dt, A, B, C, D, z, dt_bias, state, slots, softplus);
+    return Below<kScanStep, ssm_scan_step>::call(keys, x, dt, A, B, C, D, z, dt_bias, state, slots, softplus);
 }
 
 struct ConvNode : torch::autograd::Function<ConvNode> {
