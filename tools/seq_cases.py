@@ -60,7 +60,7 @@ def short(kernel):
 def summary(folder):
     _, known = cases()
     out = csv.writer(sys.stdout, lineterminator="\n")
-    out.writerow(["case", "kernel", "grid", "calls", "median_us", "min_us", "vector_busy", "vector_instructions_per_wave", "waves"])
+    out.writerow(["case", "kernel", "grid", "calls", "median_us", "min_us", "vector_busy", "vector_instructions_per_wave"])
     for case in known:
         here = os.path.join(folder, re.sub(r"\W+", "_", case["name"]))
         times, counters = {}, {}
@@ -81,8 +81,7 @@ def summary(folder):
             c = {k: sorted(v)[len(v) // 2] for k, v in counters.get((kernel, size), {}).items()}
             busy = "{:.2f}".format(c["SQ_ACTIVE_INST_VALU"] / c["SQ_BUSY_CU_CYCLES"]) if c.get("SQ_BUSY_CU_CYCLES") else ""
             per_wave = "{:.0f}".format(c["SQ_INSTS_VALU"] / c["SQ_WAVES"]) if c.get("SQ_WAVES") else ""
-            out.writerow([case["name"], kernel, grid, len(t), "{:.1f}".format(t[len(t) // 2]), "{:.1f}".format(t[0]), busy, per_wave,
-                          "{:.0f}".format(c["SQ_WAVES"]) if c else ""])
+            out.writerow([case["name"], kernel, grid, len(t), "{:.1f}".format(t[len(t) // 2]), "{:.1f}".format(t[0]), busy, per_wave])
 
 
 if __name__ == "__main__":
